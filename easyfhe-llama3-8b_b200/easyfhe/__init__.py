@@ -51,7 +51,7 @@ def get_device_module(device: str = "cuda"):
 
 def __getattr__(name):
     # fhe and bs import torch.cuda state lazily; keep `import easyfhe` cheap
-    if name in ("fhe", "bs", "core"):
+    if name in ("fhe", "bs", "core", "plain"):
         import importlib
 
         return importlib.import_module(f"{__name__}.{name}")

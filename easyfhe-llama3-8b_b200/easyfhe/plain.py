@@ -1,0 +1,434 @@
+"""Plaintext operators around an encrypted prefill, on libb200fhe's kernels.
+
+What runs in the clear beside the encrypted graph: rotary positions for the
+plain twin of a decoder layer (the reference's approx/attention.py:23-59), the
+client's head on the decrypted hidden state (final_logits, the reference's
+application/client.py:60-100) with 4-bit weights, and the score of decrypted
+hidden states against tokens with its gradient.
+
+Every call is asynchronous on the current stream of its tensors' device and
+can be captured into a CUDA graph; scratch and outputs come from torch's
+allocator on that stream.  Tensors used on a stream other than the one they
+were made on are the caller's to order, as with any torch operation.  Gradients
+are explicit calls: nothing here records an autograd graph, and tensors that
+require a gradient are refused unless gradients are switched off.  Arguments
+are checked before anything launches: ValueError for shapes, types, strides
+and devices (there is no CPU fallback).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from ._native import call, lib
+
+_DTYPES = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
+
+
+class _RopeHeads(ctypes.Structure):
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("in_batch", "in_seq", "in_head", "out_batch", "out_seq",
+                                      "out_head")] + [("heads", ctypes.c_int)]
+
+
+class _on:
+    """The device of a call: current for its launches, with its raw stream."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _check(what: str, device, **tensors) -> torch.device:
+    """Every tensor a strided CUDA tensor without a gradient, on one device."""
+
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: {name} is a {type(t).__name__}, not a tensor")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: {name} requires a gradient, which this call does not "
+                             "record (use the explicit gradient call under torch.no_grad())")
+        if t.is_conj() or t.is_neg() or t.layout != torch.strided:
+            raise ValueError(f"{what}: {name} is not a plain strided tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on a CUDA device")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+    return device
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 500000.0,
+                     scaling: dict | None = None) -> tuple[list[float], float]:
+    """Angle per position (radians) of each pair, and the factor on cos and sin.
+
+    theta^(-2i/rotary_dim), with one of the usual scalings for long contexts:
+
+    * ``{"type": "linear", "factor"}``: every frequency divided by factor;
+    * ``{"type": "bands", "factor", "low", "high", "original"}``: frequencies that
+      turn more than `high` times within the original context stay, those below
+      `low` turns are divided, those between are mixed linearly in the turns;
+    * ``{"type": "yarn", "factor", "original", "fast", "slow"}``: a ramp over the
+      pair index between the pairs that turn `fast` and `slow` times, and cos
+      and sin times 0.1 ln(factor) + 1 (or ``"attention_factor"``)."""
+
+    r = int(rotary_dim)
+    if r < 2 or r % 2:
+        raise ValueError(f"rope: {r} rotated elements (an even number)")
+    if not theta > 0 or not math.isfinite(theta):
+        raise ValueError(f"rope: theta {theta}")
+    freqs = [float(theta) ** (-2.0 * i / r) for i in range(r // 2)]
+    if scaling is None:
+        return freqs, 1.0
+    kind = scaling.get("type")
+    keys = {"linear": ("factor",), "bands": ("factor", "low", "high", "original"),
+            "yarn": ("factor", "original", "fast", "slow")}.get(kind)
+    if keys is None:
+        raise ValueError(f"rope: scaling {kind!r} not in ['bands', 'linear', 'yarn']")
+    missing = [k for k in keys if k not in scaling]
+    if missing:
+        raise ValueError(f"rope: {kind} scaling without {missing}")
+    sc = {k: float(scaling[k]) for k in keys}
+    if any(not v > 0 or not math.isfinite(v) for v in sc.values()):
+        raise ValueError(f"rope: {kind} scaling {sc}")
+    factor = sc["factor"]
+    if kind == "linear":
+        return [f / factor for f in freqs], 1.0
+    if kind == "bands":
+        if not sc["high"] > sc["low"]:
+            raise ValueError(f"rope: bands from {sc['low']} to {sc['high']} turns")
+        out = []
+        for f in freqs:
+            turns = sc["original"] * f / (2 * math.pi)
+            keep = min(max((turns - sc["low"]) / (sc["high"] - sc["low"]), 0.0), 1.0)
+            out.append((1 - keep) * f / factor + keep * f)
+        return out, 1.0
+    if not theta > 1:
+        raise ValueError(f"rope: yarn scaling with theta {theta}")
+
+    def pair(turns: float) -> float:
+        return r * math.log(sc["original"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    low = max(math.floor(pair(sc["fast"])), 0)
+    high = min(math.ceil(pair(sc["slow"])), r - 1)
+    out = []
+    for i, f in enumerate(freqs):
+        ramp = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
+        out.append(ramp * f / factor + (1 - ramp) * f)
+    return out, float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0))
+
+
+class RopePlan:
+    """Head geometry and frequencies of rotary positions, kept on one device.
+
+    ``layout``: "half" pairs element i with i + rotary_dim / 2, "interleaved"
+    2i with 2i + 1.  Elements from rotary_dim on pass through."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, theta: float = 500000.0,
+                 layout: str = "half", scaling: dict | None = None,
+                 device: str | torch.device = "cuda"):
+        self.head_dim = int(head_dim)
+        self.rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
+        if not 2 <= self.head_dim <= 1024 or not 2 <= self.rotary_dim <= self.head_dim:
+            raise ValueError(f"rope: {self.rotary_dim} rotated of {self.head_dim} elements "
+                             "(2 up to the head's, heads of up to 1024)")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"rope: layout {layout!r} not in ['half', 'interleaved']")
+        self.layout = layout
+        freqs, self.factor = rope_frequencies(self.rotary_dim, theta, scaling)
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError("rope: libb200fhe runs on CUDA devices only (no CPU fallback)")
+        self.freqs = torch.tensor(freqs, dtype=torch.float64, device=dev)
+        self.device = self.freqs.device
+
+
+def _rope(what, q, k, positions, plan, gradient):
+    if not isinstance(plan, RopePlan):
+        raise ValueError(f"{what}: plan is a {type(plan).__name__}")
+    dev = _check(what, plan.device, q=q, k=k, positions=positions)
+    parts = [q] if k is None else [q, k]
+    for name, t in zip("qk", parts):
+        if t.dim() not in (3, 4) or t.shape[-1] != plan.head_dim:
+            raise ValueError(f"{what}: {name} of shape {tuple(t.shape)}, expected [(batch,) seq, "
+                             f"heads, {plan.head_dim}]")
+        if t.dtype not in _DTYPES or t.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} is {t.dtype}")
+        if t.shape[:-2] != q.shape[:-2]:
+            raise ValueError(f"{what}: {name} of shape {tuple(t.shape)} beside q of "
+                             f"{tuple(q.shape)}")
+        if not 1 <= t.shape[-2] <= 4096:
+            raise ValueError(f"{what}: {name} has {t.shape[-2]} heads (1 to 4096)")
+    batch, seq = (1, q.shape[0]) if q.dim() == 3 else (q.shape[0], q.shape[1])
+    if positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what}: positions are {positions.dtype} (int64 or int32)")
+    if tuple(positions.shape) not in ((seq,), (batch, seq)):
+        raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} for {batch} x "
+                         f"{seq} tokens")
+    pos_b = positions.stride(0) if positions.dim() == 2 else 0
+    parts = [t if t.stride(-1) == 1 else t.contiguous() for t in parts]
+    res = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in parts]
+    arr = (_RopeHeads * len(parts))()
+    for i, (t, o) in enumerate(zip(parts, res)):
+        ib = t.stride(0) if t.dim() == 4 else 0
+        ob = o.stride(0) if t.dim() == 4 else 0
+        arr[i] = _RopeHeads(t.data_ptr(), o.data_ptr(), ib, t.stride(-3), t.stride(-2), ob,
+                            o.stride(-3), o.stride(-2), t.shape[-2])
+    if batch and seq:
+        with _on(dev) as stream:
+            call("b2f_rope", ctypes.addressof(arr), len(parts), _DTYPES[q.dtype], batch, seq,
+                 plan.head_dim, plan.rotary_dim, int(plan.layout == "interleaved"),
+                 positions.data_ptr(), int(positions.dtype == torch.int64), pos_b,
+                 positions.stride(-1), plan.freqs.data_ptr(), float(plan.factor),
+                 int(gradient), stream)
+    return res[0] if k is None else (res[0], res[1])
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Tensor,
+         plan: RopePlan):
+    """Rotary positions of q, or of q and k in one launch.
+
+    q, k: [seq, heads, head_dim] or [batch, seq, heads, head_dim] (f64, f32, f16
+    or bf16; strides free, a last one other than 1 costs a copy), positions
+    [seq] or [batch, seq] (int64 or int32).  Returns contiguous tensors.  Angles
+    are taken in binary64, products in binary32 (binary64 for f64)."""
+
+    return _rope("rope", q, k, positions, plan, False)
+
+
+def rope_grad(grad_q: torch.Tensor, grad_k: torch.Tensor | None = None, *,
+              positions: torch.Tensor, plan: RopePlan):
+    """The gradient of `rope`: the rotation by the negative angle."""
+
+    return _rope("rope_grad", grad_q, grad_k, positions, plan, True)
+
+
+# ---------------------------------------------------------------------------
+# matrix-vector products with 4-bit weights
+# ---------------------------------------------------------------------------
+
+
+class Q4Weight:
+    """A 4-bit weight [rows, cols] laid out for `q4_matvec` (`pack_q4`,
+    `quantize_q4`): scale * (code - zero) per group of columns."""
+
+    def __init__(self, shape, group, packed, scales, scale_dtype, zeros):
+        self.shape = (int(shape[0]), int(shape[1]))
+        self.group = int(group)
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.scale_dtype = scale_dtype
+        self.device = packed.device
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size()
+                   for t in (self.packed, self.scales, self.zeros) if t is not None)
+
+
+def _group(what: str, group: int, cols: int) -> int:
+    group = int(group)
+    if group != 32 and (group < 64 or group % 64):
+        raise ValueError(f"{what}: groups of {group} columns (32 or a multiple of 64)")
+    return -(-cols // group)
+
+
+def pack_q4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+            group: int = 128) -> Q4Weight:
+    """Lay out codes [rows, cols] (uint8, 0..15) with scales and zero points
+    (uint8, 0..15; none: 8) [rows, ceil(cols / group)] for `q4_matvec`.  Done
+    once per weight: it waits for the device to check the codes."""
+
+    dev = _check("pack_q4", None, codes=codes, scales=scales, zeros=zeros)
+    if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.numel():
+        raise ValueError(f"pack_q4: codes of shape {tuple(codes.shape)}, {codes.dtype}")
+    n, k = codes.shape
+    groups = _group("pack_q4", group, k)
+    if tuple(scales.shape) != (n, groups) or scales.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"pack_q4: scales of shape {tuple(scales.shape)}, {scales.dtype}, "
+                         f"expected [{n}, {groups}] in float16 or bfloat16")
+    if zeros is not None and (tuple(zeros.shape) != (n, groups) or zeros.dtype != torch.uint8):
+        raise ValueError(f"pack_q4: zeros of shape {tuple(zeros.shape)}, {zeros.dtype}")
+    for name, t in (("codes", codes), ("zeros", zeros)):
+        if t is not None and int(t.max()) > 15:
+            raise ValueError(f"pack_q4: {name} above 15")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    rows16 = -(-n // 16) * 16
+    packed = torch.empty(lib.b2f_q4_packed_bytes(n, k), dtype=torch.uint8, device=dev)
+    ps = torch.empty(rows16 * groups, dtype=scales.dtype, device=dev)
+    pz = None if zeros is None else torch.empty(rows16 * groups, dtype=torch.uint8, device=dev)
+    with _on(dev) as stream:
+        call("b2f_q4_pack", codes.data_ptr(), scales.data_ptr(),
+             None if zeros is None else zeros.data_ptr(), n, k, int(group), packed.data_ptr(),
+             ps.data_ptr(), None if pz is None else pz.data_ptr(), stream)
+    return Q4Weight((n, k), group, packed, ps, scales.dtype, pz)
+
+
+def q4_codes(weight: torch.Tensor, *, group: int = 128, symmetric: bool = True,
+             scale_dtype: torch.dtype = torch.bfloat16):
+    """Codes, scales and zero points (None when symmetric) of a finite weight
+    [rows, cols] (f32, f16 or bf16): round to nearest against the stored scale,
+    max|w| / 7 of a group, or its range in 15 steps with an integer zero."""
+
+    dev = _check("q4_codes", None, weight=weight)
+    if weight.dim() != 2 or not weight.numel() or _DTYPES.get(weight.dtype, 0) == 0:
+        raise ValueError(f"q4_codes: weight of shape {tuple(weight.shape)}, {weight.dtype}")
+    if scale_dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"q4_codes: scales in {scale_dtype} (float16 or bfloat16)")
+    n, k = weight.shape
+    groups = _group("q4_codes", group, k)
+    w = weight if weight.stride(1) == 1 and weight.stride(0) >= k else weight.contiguous()
+    codes = torch.empty((n, k), dtype=torch.uint8, device=dev)
+    scales = torch.empty((n, groups), dtype=scale_dtype, device=dev)
+    zeros = None if symmetric else torch.empty((n, groups), dtype=torch.uint8, device=dev)
+    with _on(dev) as stream:
+        call("b2f_q4_quantize", w.data_ptr(), _DTYPES[w.dtype], max(w.stride(0), k), n, k,
+             int(group), int(bool(symmetric)), _DTYPES[scale_dtype], codes.data_ptr(),
+             scales.data_ptr(), None if zeros is None else zeros.data_ptr(), stream)
+    return codes, scales, zeros
+
+
+def quantize_q4(weight: torch.Tensor, *, group: int = 128, symmetric: bool = True,
+                scale_dtype: torch.dtype = torch.bfloat16) -> Q4Weight:
+    """A weight in 4 bits, laid out for `q4_matvec` (`q4_codes` + `pack_q4`)."""
+
+    codes, scales, zeros = q4_codes(weight, group=group, symmetric=symmetric,
+                                    scale_dtype=scale_dtype)
+    return pack_q4(codes, scales, zeros, group=group)
+
+
+def q4_matvec(x: torch.Tensor, weight: Q4Weight, *,
+              out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """x [..., cols] times the weight's transpose: [..., rows], up to 1024 rows
+    of x (f32, f16 or bf16; f32 keeps its 24 bits), summed in binary32.  Returns
+    x's type, or float32 with ``out_dtype=torch.float32``."""
+
+    if not isinstance(weight, Q4Weight):
+        raise ValueError(f"q4_matvec: weight is a {type(weight).__name__}")
+    dev = _check("q4_matvec", weight.device, x=x)
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k or _DTYPES.get(x.dtype, 0) == 0:
+        raise ValueError(f"q4_matvec: x of shape {tuple(x.shape)}, {x.dtype}, for {k} columns")
+    if out_dtype not in (None, x.dtype, torch.float32):
+        raise ValueError(f"q4_matvec: output in {out_dtype} for x in {x.dtype}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    rows = x.numel() // k
+    if rows > 1024:
+        raise ValueError(f"q4_matvec: {rows} rows (up to 1024)")
+    x2 = x if x.dim() == 2 else x.reshape(rows, k)
+    if x2.stride(1) != 1 and k > 1 or rows > 1 and x2.stride(0) < k:
+        x2 = x2.contiguous()
+    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=dev)
+    if rows:
+        with _on(dev) as stream:
+            call("b2f_q4_matvec", x2.data_ptr(), _DTYPES[x.dtype],
+                 x2.stride(0) if rows > 1 else k, rows, weight.packed.data_ptr(),
+                 weight.scales.data_ptr(), _DTYPES[weight.scale_dtype],
+                 None if weight.zeros is None else weight.zeros.data_ptr(), n, k, weight.group,
+                 y.data_ptr(), int(out_dtype == torch.float32), stream)
+    return y
+
+
+# ---------------------------------------------------------------------------
+# cross entropy over the vocabulary
+# ---------------------------------------------------------------------------
+
+
+def _loss_args(what, hidden, weight, labels):
+    dev = _check(what, None, hidden=hidden, weight=weight, labels=labels)
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError(f"{what}: hidden of shape {tuple(hidden.shape)}, weight of "
+                         f"{tuple(weight.shape)}")
+    if hidden.dtype not in (torch.float16, torch.bfloat16) or weight.dtype != hidden.dtype:
+        raise ValueError(f"{what}: hidden is {hidden.dtype}, weight {weight.dtype} (both "
+                         "float16 or both bfloat16)")
+    t, d = hidden.shape
+    if d % 8 or not d or not weight.shape[0]:
+        raise ValueError(f"{what}: weight of shape {tuple(weight.shape)} (a hidden size that is "
+                         "a multiple of 8, at least one word)")
+    if labels.dtype != torch.int64 or tuple(labels.shape) != (t,):
+        raise ValueError(f"{what}: labels of shape {tuple(labels.shape)}, {labels.dtype}, for "
+                         f"{t} tokens (int64)")
+
+    def rows(m):  # as TMA reads it: 16-byte aligned rows
+        ok = m.stride(1) == 1 and m.stride(0) >= d and m.stride(0) % 8 == 0 \
+            and m.data_ptr() % 16 == 0
+        return m if ok else m.clone(memory_format=torch.contiguous_format)
+
+    return dev, rows(hidden), rows(weight), labels.contiguous()
+
+
+def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *,
+               ignore_index: int = -100) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cross entropy of softmax(hidden @ weight.T) against labels, per token,
+    without the logits: (loss [tokens], lse [tokens]) in float32.
+
+    hidden [tokens, D], weight [words, D] (both f16 or both bf16, D a multiple
+    of 8), labels int64.  A label of ignore_index gives 0; any other label
+    outside the vocabulary gives NaN, as do logits that overflow."""
+
+    dev, h, w, lab = _loss_args("vocab_loss", hidden, weight, labels)
+    t, d = h.shape
+    v = w.shape[0]
+    loss = torch.empty(t, dtype=torch.float32, device=dev)
+    lse = torch.empty(t, dtype=torch.float32, device=dev)
+    if t:
+        ws = torch.empty(lib.b2f_vocab_loss_workspace(t, v), dtype=torch.uint8, device=dev)
+        with _on(dev) as stream:
+            call("b2f_vocab_loss", h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
+                 _DTYPES[h.dtype], t, v, d, lab.data_ptr(), int(ignore_index), loss.data_ptr(),
+                 lse.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    return loss, lse
+
+
+def vocab_loss_grad(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
+                    lse: torch.Tensor, grad_loss: torch.Tensor, *, ignore_index: int = -100,
+                    need_hidden: bool = True, need_weight: bool = True):
+    """The gradient of `vocab_loss` for grad_loss [tokens] (float32), from the
+    lse it returned for the same inputs: (grad_hidden, grad_weight) in the
+    operands' type, None for one that is not needed.
+
+    The logits are computed again in pieces of the vocabulary.  Rows of ignored
+    tokens contribute nothing and get zero, whatever they hold."""
+
+    what = "vocab_loss_grad"
+    dev, h, w, lab = _loss_args(what, hidden, weight, labels)
+    _check(what, dev, lse=lse, grad_loss=grad_loss)
+    t, d = h.shape
+    v = w.shape[0]
+    for name, x in (("lse", lse), ("grad_loss", grad_loss)):
+        if x.dtype != torch.float32 or tuple(x.shape) != (t,):
+            raise ValueError(f"{what}: {name} of shape {tuple(x.shape)}, {x.dtype}, for {t} "
+                             "tokens (float32)")
+    if not (need_hidden or need_weight):
+        raise ValueError(f"{what}: no gradient asked for")
+    lse, g = lse.contiguous(), grad_loss.contiguous()
+    dh = torch.empty((t, d), dtype=h.dtype, device=dev) if need_hidden else None
+    dw = torch.empty((v, d), dtype=w.dtype, device=dev) if need_weight else None
+    with _on(dev) as stream:
+        ws = torch.empty(max(lib.b2f_vocab_loss_grad_workspace(t, v, d, int(need_hidden)), 16),
+                         dtype=torch.uint8, device=dev)
+        call("b2f_vocab_loss_grad", h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
+             _DTYPES[h.dtype], t, v, d, lab.data_ptr(), int(ignore_index), lse.data_ptr(),
+             g.data_ptr(), None if dh is None else dh.data_ptr(),
+             None if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    return dh, dw

@@ -466,6 +466,84 @@ int b2f_decrypt(b2f_context *ctx, const uint64_t *ct, int l,
  * host output, same ChaCha20 stream definition as the keys. */
 int b2f_sample_secret(int log_n, uint64_t seed, int hamming, int8_t *s_out);
 
+/* ---- plaintext operators around an encrypted prefill ----
+ * What runs in the clear beside the encrypted graph: the plain twin of a
+ * decoder layer (rotary positions, llama3fhe/approx/attention.py:23-59) and
+ * the client's head on decrypted hidden states (final_logits,
+ * llama3fhe/application/client.py:60-100).  These calls take no context: all
+ * buffers lie on the current device, and the workspaces are required (a null
+ * one is refused).  Element types: */
+enum { B2F_F64 = 0, B2F_F32 = 1, B2F_F16 = 2, B2F_BF16 = 3 };
+
+/* Heads of one tensor [batch][seq][heads][dim], strides in elements, the last
+ * dimension contiguous.  out may be in with the same strides (in place);
+ * otherwise they must not overlap. */
+typedef struct {
+  const void *in;
+  void *out;
+  int64_t in_batch, in_seq, in_head;
+  int64_t out_batch, out_seq, out_head;
+  int heads;
+} b2f_rope_heads;
+/* Rotary positions of one or two tensors (queries and keys) in one launch.
+ * Pair i < rotary / 2 of a head, elements (i, i + rotary / 2) or, interleaved,
+ * (2i, 2i + 1), turns by positions[b][s] * freqs[i] (radians) and is scaled by
+ * factor; elements from rotary on are copied.  gradient: by the negative
+ * angle.  positions: int64 (positions64) or int32, strides in elements. */
+int b2f_rope(const b2f_rope_heads *parts, int num_parts, int dtype, int64_t batch,
+             int64_t seq, int dim, int rotary, int interleaved, const void *positions,
+             int positions64, int64_t pos_batch_stride, int64_t pos_seq_stride,
+             const double *freqs, double factor, int gradient, void *stream);
+
+/* 4-bit weights [N][K] with a scale (fp16 or bf16) and optionally a zero point
+ * per row and group of `group` columns (32 or a multiple of 64; the last one
+ * may be cut short): weight = scale * (code - zero), code 0..15, zero 8
+ * without zero points.  Packed: b2f_q4_packed_bytes of codes, scales and zero
+ * points of ceil(N / 16) * 16 rows (2 and 1 bytes each). */
+size_t b2f_q4_packed_bytes(int64_t N, int64_t K);
+/* codes [N][K] (one byte each, 0..15), scales and zeros [N][groups]; zeros and
+ * packed_zeros are null for zero 8. */
+int b2f_q4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t N,
+                int64_t K, int group, void *packed, void *packed_scales, void *packed_zeros,
+                void *stream);
+/* Codes, scales and zero points of a weight (f32, f16 or bf16, rows ld apart):
+ * symmetric: scale max|w| / 7, code round(w / scale) + 8 (zeros null);
+ * otherwise [min(w, 0), max(w, 0)] in 15 steps.  Finite weights. */
+int b2f_q4_quantize(const void *w, int dtype, int64_t ld, int64_t N, int64_t K, int group,
+                    int symmetric, int scale_dtype, uint8_t *codes, void *scales,
+                    uint8_t *zeros, void *stream);
+/* y[b][n] = sum_k weight[n][k] x[b][k] of up to 1024 rows of x (f32, f16 or
+ * bf16, rows ldx apart), summed in binary32; y [rows][N] in x's type, or
+ * binary32 with out_f32.  The weight is read once per 32 rows (10 of f32). */
+int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const void *packed,
+                  const void *scales, int scale_dtype, const void *zeros, int64_t N, int64_t K,
+                  int group, void *y, int out_f32, void *stream);
+
+/* Softmax cross entropy of logits hidden [T][D] x weight [V][D]^T (fp16 or
+ * bf16, rows ldh / ldw apart, D and both strides multiples of 8, 16-byte
+ * aligned) against labels [T], without the logits being kept: lse[t] = log sum_v
+ * exp z_tv, loss[t] = lse[t] - z_{t, label}; 0 where the label is `ignore`, NaN
+ * where it is any other value outside [0, V).  Workspace 256-byte aligned. */
+size_t b2f_vocab_loss_workspace(int64_t T, int64_t V);
+int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int dtype,
+                   int64_t T, int64_t V, int64_t D, const int64_t *labels, int64_t ignore,
+                   float *loss, float *lse, void *ws, size_t ws_bytes, void *stream);
+/* Its gradient for grad_loss [T] with the lse that b2f_vocab_loss returned for
+ * the same inputs: grad_hidden [T][D] and / or grad_weight [V][D] (contiguous,
+ * in the operands' type; null: not computed).  Rows of ignored tokens
+ * contribute nothing, whatever they hold, and get zero.  The workspace query
+ * is for the current device. */
+size_t b2f_vocab_loss_grad_workspace(int64_t T, int64_t V, int64_t D, int need_hidden);
+int b2f_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw,
+                        int dtype, int64_t T, int64_t V, int64_t D, const int64_t *labels,
+                        int64_t ignore, const float *lse, const float *grad_loss,
+                        void *grad_hidden, void *grad_weight, void *ws, size_t ws_bytes,
+                        void *stream);
+/* Waits of the two calls above that ran out (the block ended, its outputs are
+ * not written) since the library loaded, on the current device; 0 on a
+ * healthy run, -1 when the counter cannot be read. */
+int b2f_vocab_loss_wait_errors(void);
+
 #ifdef __cplusplus
 }
 #endif
