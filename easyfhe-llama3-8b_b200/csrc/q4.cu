@@ -24,6 +24,15 @@
 //
 // Rows in binary32 are split into three truncations to bf16 (8 + 8 + 8 bits:
 // exact), each its own column of the product, and joined at the end.
+//
+// A cluster of 1, 2, 4 or 8 blocks shares a row block: the columns are split over
+// the blocks (as many as it takes for x to fit shared memory), and over a
+// block's warps in chunks of a few tiles.  x is laid out in shared memory once
+// per block, in operand order, so a tile costs two 16-byte reads of it.  Every
+// warp keeps the weights of its next chunk in flight in registers (a register
+// is refilled as soon as its tile is done).  The warps' sums of a row block meet
+// in shared memory, two buffers and one barrier per row block, and are added in
+// a fixed order.
 #include "b2f_internal.h"
 
 #include <cuda_bf16.h>
@@ -43,8 +52,14 @@ struct Q4Args {
   const void *x;
   void *y;
   long long ldx, ldy;
-  int N, K, tiles_k, groups, group_tiles;  // group_tiles: 64-column tiles of a group, 0 for 32
-  int rows, out_f32, x_vec, per_warp;
+  int N, K, tiles_k, groups;
+  int group_tiles;          // 64-column tiles of a group, 0 for groups of 32
+  // ceil(2^32 / group_tiles), tile / group_tiles in one product (both below 2^14: exact);
+  // 0 for groups of one tile
+  uint32_t group_magic;
+  int rows, cols, out_f32, x_vec, scale_bf16;
+  int block_tiles;          // tiles of x of one block of a cluster
+  int warps, cluster;
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -62,6 +77,15 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// d = a b
+template <class T>
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1, T t) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = 0.0f;
+  mma_16816(d, a, b0, b1, t);
 }
 
 // two nibbles (bits 0-3 and 16-19 of w) -> code - z in both halves; base is
@@ -84,9 +108,8 @@ __device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t bz, __half) {
   return *reinterpret_cast<const uint32_t *>(&d);
 }
 
-template <bool SB>
-__device__ __forceinline__ float2 scale_pair(uint32_t v) {
-  if (SB) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+__device__ __forceinline__ float2 scale_pair(uint32_t v, int bf16) {
+  if (bf16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
@@ -132,98 +155,179 @@ __device__ __forceinline__ uint2 load_x(const Q4Args &a, int col, int k) {
   }
 }
 
-// One block: row blocks blockIdx.x, + gridDim.x, ...; warp w sums tiles
-// [w per_warp, (w + 1) per_warp) of a row block, then the block adds the
-// warps' sums in order.  NT: 8-column tiles of x (planes counted).
-template <class T, bool SPLIT, int NT, bool ZERO, bool SB>
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float remote_f32(const float *p, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n"
+               : "=r"(a)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+// a barrier of the block, or of its cluster of cs blocks
+__device__ __forceinline__ void meet(int cs) {
+  if (cs == 1) {
+    __syncthreads();
+  } else {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  }
+}
+
+// Cluster c of gridDim.x / cs takes row blocks c, c + clusters, ...; block r of a
+// cluster takes tiles [r block_tiles, (r + 1) block_tiles), its warp w the chunks
+// of TPW tiles w, w + warps, ... of those.  NT: 8-column tiles of x (planes
+// counted).  Shared memory: x [block_tiles][2][cols][4 lanes] of 16 bytes, then
+// two buffers of sums [warps][16][8 NT].
+template <class T, bool SPLIT, int NT, int TPW, bool ZERO, bool G32>
 __global__ void __launch_bounds__(32 * Q4_MAX_WARPS)
     q4_matvec_kernel(const Q4Args a) {
-  extern __shared__ float q4_sums[];  // [warps][16][8 NT]
+  extern __shared__ __align__(16) unsigned char q4_smem[];
+  uint4 *xs = reinterpret_cast<uint4 *>(q4_smem);
+  float *sums = reinterpret_cast<float *>(q4_smem + (size_t)a.block_tiles * a.cols * 128);
+  constexpr int SUMS = Q4_ROWS * 8 * NT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int cs = a.cluster, rank = cs == 1 ? 0 : (int)cluster_rank();
   const int row_blocks = (a.N + Q4_ROWS - 1) / Q4_ROWS;
-  const int k_begin = warp * a.per_warp, k_end = min(k_begin + a.per_warp, a.tiles_k);
-  for (int rb = blockIdx.x; rb < row_blocks; rb += gridDim.x) {
-    const uint4 *wp = a.packed + ((long long)rb * a.tiles_k) * 32 + lane;
-    const uint32_t *sp = a.scales + (long long)rb * a.groups * 8 + g;
-    const uint16_t *zp = ZERO ? a.zeros + (long long)rb * a.groups * 8 + g : nullptr;
-    float tot[NT][4], acc[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tot[j][i] = acc[j][i] = 0.0f;
-    uint32_t bz0 = kNibbleBase<T> + 0x00080008u, bz1 = bz0;
-    auto zero_of = [&](int grp) {
-      if (!ZERO) return;
-      const uint32_t z = __ldg(zp + grp * 8);
-      bz0 = kNibbleBase<T> + (z & 0xff) * 0x00010001u;
-      bz1 = kNibbleBase<T> + (z >> 8) * 0x00010001u;
-    };
-    // apply the group's scales to its sums and start the next group
-    auto flush = [&](int grp) {
-      const float2 s = scale_pair<SB>(__ldg(sp + grp * 8));
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        tot[j][0] += s.x * acc[j][0];
-        tot[j][1] += s.x * acc[j][1];
-        tot[j][2] += s.y * acc[j][2];
-        tot[j][3] += s.y * acc[j][3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+  const int stride = gridDim.x / cs;
+  const int tile0 = rank * a.block_tiles;
+  const int tiles = max(0, min(a.block_tiles, a.tiles_k - tile0));
+  const int chunks = (tiles + TPW - 1) / TPW;
+
+  int rb = blockIdx.x / cs, chunk = warp;
+  uint4 w[TPW];
+  uint32_t sc[G32 ? 2 * TPW : TPW];
+  uint16_t zr[ZERO ? (G32 ? 2 * TPW : TPW) : 1];
+  // tile i of a chunk into its registers (zeros past the block's tiles)
+  auto fetch = [&](int i, int r, int c) {
+    const int kt = c * TPW + i;
+    const bool in = r < row_blocks && kt < tiles;
+    const int k = tile0 + kt;
+    w[i] = in ? __ldcs(a.packed + ((long long)r * a.tiles_k + k) * 32 + lane)
+              : make_uint4(0, 0, 0, 0);
+    const int grp = G32 ? 2 * k : a.group_magic ? (int)__umulhi((uint32_t)k, a.group_magic) : k;
+    const long long at = ((long long)r * a.groups + grp) * 8 + g;
+    if (G32) {
+      const bool two = in && grp + 1 < a.groups;
+      sc[2 * i] = in ? __ldg(a.scales + at) : 0;
+      sc[2 * i + 1] = two ? __ldg(a.scales + at + 8) : 0;
+      if (ZERO) {
+        zr[2 * i] = in ? __ldg(a.zeros + at) : 0;
+        zr[2 * i + 1] = two ? __ldg(a.zeros + at + 8) : 0;
       }
-    };
-    for (int kt = k_begin; kt < k_end; ++kt) {
-      const uint4 w4 = __ldg(wp + (long long)kt * 32);
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-      const int grp = a.group_tiles ? kt / a.group_tiles : 2 * kt;
-      zero_of(grp);
+    } else {
+      sc[i] = in ? __ldg(a.scales + at) : 0;
+      if (ZERO) zr[i] = in ? __ldg(a.zeros + at) : 0;
+    }
+  };
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (m == 2 && !a.group_tiles) {  // groups of 32: two per tile
-          flush(grp);
-          if (grp + 1 >= a.groups) break;  // columns past K
-          zero_of(grp + 1);
-        }
-        uint32_t f[4];
-        f[0] = nibbles(w[m], bz0, T());
-        f[1] = nibbles(w[m] >> 4, bz1, T());
-        f[2] = nibbles(w[m] >> 8, bz0, T());
-        f[3] = nibbles(w[m] >> 12, bz1, T());
+  for (int i = 0; i < TPW; ++i) fetch(i, rb, chunk);
+
+  for (int i = threadIdx.x; i < tiles * a.cols * 4; i += blockDim.x) {
+    const int q = i & 3, c = (i >> 2) % a.cols, kt = (i >> 2) / a.cols;
+    const int k = (tile0 + kt) * Q4_COLS + 4 * q;
+    uint4 *o = xs + ((size_t)kt * 2 * a.cols + c) * 4 + q;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint2 lo = load_x<T, SPLIT>(a, c, k + 32 * h);
+      const uint2 hi = load_x<T, SPLIT>(a, c, k + 32 * h + 16);
+      o[h * a.cols * 4] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+  }
+  __syncthreads();
+
+  float tot[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tot[j][i] = 0.0f;
+
+  for (int buf = 0; rb < row_blocks; buf ^= 1) {
+    for (; chunk < chunks;) {
+      int next = chunk + warps, next_rb = rb;
+      if (next >= chunks) next = warp, next_rb = rb + stride;
+#pragma unroll
+      for (int i = 0; i < TPW; ++i) {
+        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        const int kt = chunk * TPW + i;
+        uint4 xv[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const uint2 b = load_x<T, SPLIT>(a, 8 * j + g, kt * Q4_COLS + 16 * m + 4 * t);
-          mma_16816(acc[j], f, b.x, b.y, T());
+          const bool on = 8 * j + g < a.cols && kt < tiles;
+          const uint4 *xp = xs + ((size_t)kt * 2 * a.cols + 8 * j + g) * 4 + t;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            xv[j][h] = on ? xp[h * a.cols * 4] : make_uint4(0, 0, 0, 0);
         }
+        float acc[NT][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int si = G32 ? 2 * i + m / 2 : i;
+          uint32_t bz0 = kNibbleBase<T> + 0x00080008u, bz1 = bz0;
+          if (ZERO) {
+            bz0 = kNibbleBase<T> + (zr[ZERO ? si : 0] & 0xffu) * 0x00010001u;
+            bz1 = kNibbleBase<T> + (uint32_t)(zr[ZERO ? si : 0] >> 8) * 0x00010001u;
+          }
+          uint32_t f[4];
+          f[0] = nibbles(v[m], bz0, T());
+          f[1] = nibbles(v[m] >> 4, bz1, T());
+          f[2] = nibbles(v[m] >> 8, bz0, T());
+          f[3] = nibbles(v[m] >> 12, bz1, T());
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint32_t b0 = m & 1 ? xv[j][m / 2].z : xv[j][m / 2].x;
+            const uint32_t b1 = m & 1 ? xv[j][m / 2].w : xv[j][m / 2].y;
+            if (m == 0 || (G32 && m == 2))
+              mma_first(acc[j], f, b0, b1, T());
+            else
+              mma_16816(acc[j], f, b0, b1, T());
+          }
+          if (m == 3 || (G32 && m == 1)) {  // the group's (or the tile's part of its) sums
+            const float2 s = scale_pair(sc[si], a.scale_bf16);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              tot[j][0] += s.x * acc[j][0];
+              tot[j][1] += s.x * acc[j][1];
+              tot[j][2] += s.y * acc[j][2];
+              tot[j][3] += s.y * acc[j][3];
+            }
+          }
+        }
+        fetch(i, next_rb, next);
       }
-      if (!a.group_tiles) {
-        if (grp + 1 < a.groups) flush(grp + 1);
-      } else if (kt + 1 == k_end || (kt + 1) % a.group_tiles == 0) {
-        flush(grp);
-      }
+      chunk += warps;
     }
+    chunk = warp;
     // c0, c1: row g, columns 2t, 2t + 1; c2, c3: row g + 8
-    float *out = q4_sums + warp * (Q4_ROWS * 8 * NT);
+    float *out = sums + (buf * warps + warp) * SUMS;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       float *o = out + g * 8 * NT + 8 * j + 2 * t;
-      o[0] = tot[j][0], o[1] = tot[j][1];
-      o[8 * 8 * NT] = tot[j][2], o[8 * 8 * NT + 1] = tot[j][3];
+      *reinterpret_cast<float2 *>(o) = make_float2(tot[j][0], tot[j][1]);
+      *reinterpret_cast<float2 *>(o + 8 * 8 * NT) = make_float2(tot[j][2], tot[j][3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tot[j][i] = 0.0f;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < Q4_ROWS * a.rows; i += blockDim.x) {
+    meet(cs);
+    for (int i = threadIdx.x + rank * blockDim.x; i < Q4_ROWS * a.rows; i += cs * blockDim.x) {
       const int r = i & 15, b = i >> 4, n = rb * Q4_ROWS + r;
       if (n < a.N) {
         float v = 0.0f;
-        for (int w = 0; w < warps; ++w) {
-          const float *s = q4_sums + (w * Q4_ROWS + r) * 8 * NT;
-          if (SPLIT) {
-            // the small planes first
-            const float lo = s[3 * b + 2] + s[3 * b + 1];
-            v += s[3 * b] + lo;
-          } else {
-            v += s[b];
+        for (int c = 0; c < cs; ++c)
+          for (int u = 0; u < warps; ++u) {
+            const float *s = sums + (buf * warps + u) * SUMS + r * 8 * NT;
+            auto at = [&](int col) { return cs == 1 ? s[col] : remote_f32(s + col, c); };
+            if (SPLIT)
+              v += at(3 * b) + (at(3 * b + 2) + at(3 * b + 1));
+            else
+              v += at(b);
           }
-        }
         const long long at = b * a.ldy + n;
         if (SPLIT || a.out_f32)
           static_cast<float *>(a.y)[at] = v;
@@ -231,8 +335,9 @@ __global__ void __launch_bounds__(32 * Q4_MAX_WARPS)
           static_cast<T *>(a.y)[at] = (T)v;
       }
     }
-    __syncthreads();
+    rb += stride;
   }
+  if (cs > 1) meet(cs);  // no block leaves while its sums are read
 }
 
 // codes [N][K] (one byte each) -> tiles; pairs of scales and zero points
@@ -312,27 +417,60 @@ __global__ void q4_quantize_kernel(const T *__restrict__ w, long long ld, int N,
   }
 }
 
-template <class T, bool SPLIT, int NT>
-int launch_matvec(const Q4Args &a, bool zero, bool sb, int grid, int warps, cudaStream_t s) {
-  const size_t smem = (size_t)warps * Q4_ROWS * 8 * NT * sizeof(float);
-  auto go = [&](auto kernel) { kernel<<<grid, 32 * warps, smem, s>>>(a); };
-  if (zero && sb)
-    go(q4_matvec_kernel<T, SPLIT, NT, true, true>);
-  else if (zero)
-    go(q4_matvec_kernel<T, SPLIT, NT, true, false>);
-  else if (sb)
-    go(q4_matvec_kernel<T, SPLIT, NT, false, true>);
-  else
-    go(q4_matvec_kernel<T, SPLIT, NT, false, false>);
+constexpr size_t kQ4Smem = 227 * 1024;
+
+size_t smem_bytes(const Q4Args &a, int nt) {
+  return (size_t)a.block_tiles * a.cols * 128 + (size_t)2 * a.warps * Q4_ROWS * 8 * nt * 4;
+}
+
+template <class T, bool SPLIT, int NT, bool ZERO, bool G32>
+int launch_matvec(Q4Args a, int sms, cudaStream_t s) {
+  constexpr int TPW = NT > 1 || G32 ? 4 : 8;
+  auto k = q4_matvec_kernel<T, SPLIT, NT, TPW, ZERO, G32>;
+  // the fewest blocks whose shares of x fit shared memory
+  size_t smem = 0;
+  for (a.cluster = 1; a.cluster <= 8; a.cluster *= 2) {
+    a.block_tiles = (a.tiles_k + a.cluster - 1) / a.cluster;
+    const int chunks = (a.block_tiles + TPW - 1) / TPW;
+    const int visits = (chunks + Q4_MAX_WARPS - 1) / Q4_MAX_WARPS;
+    a.warps = (chunks + visits - 1) / visits;
+    smem = (size_t)a.block_tiles * a.cols * 128 + (size_t)2 * a.warps * Q4_ROWS * 8 * NT * 4;
+    if (smem <= kQ4Smem) break;
+  }
+  B2F_CHECK_ARG(a.cluster <= 8, "b2f_q4_matvec: %d columns of %d values do not fit", a.cols, a.K);
+  B2F_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQ4Smem));
+  const int row_blocks = (a.N + Q4_ROWS - 1) / Q4_ROWS;
+  // blocks of an SM: by shared memory and by 16 warps (128 registers a thread)
+  const int per_sm = std::max(1, std::min<int>((int)(kQ4Smem / (smem + 1024)), 16 / a.warps));
+  const int clusters = std::min(row_blocks, std::max(1, sms * per_sm / a.cluster));
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(clusters * a.cluster);
+  c.blockDim = dim3(32 * a.warps);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = a.cluster > 1 ? 1 : 0;
+  B2F_CUDA(cudaLaunchKernelEx(&c, k, a));
   B2F_LAUNCHED("q4_matvec_kernel");
   return B2F_OK;
 }
+template <class T, bool SPLIT, int NT>
+int launch_cols(const Q4Args &a, int sms, cudaStream_t s) {
+  if (a.zeros)
+    return a.group_tiles ? launch_matvec<T, SPLIT, NT, true, false>(a, sms, s)
+                         : launch_matvec<T, SPLIT, NT, true, true>(a, sms, s);
+  return a.group_tiles ? launch_matvec<T, SPLIT, NT, false, false>(a, sms, s)
+                       : launch_matvec<T, SPLIT, NT, false, true>(a, sms, s);
+}
 template <class T, bool SPLIT>
-int launch_matvec_cols(const Q4Args &a, int cols, bool zero, bool sb, int grid, int warps,
-                       cudaStream_t s) {
-  if (cols <= 8) return launch_matvec<T, SPLIT, 1>(a, zero, sb, grid, warps, s);
-  if (cols <= 16) return launch_matvec<T, SPLIT, 2>(a, zero, sb, grid, warps, s);
-  return launch_matvec<T, SPLIT, 4>(a, zero, sb, grid, warps, s);
+int launch_rows(const Q4Args &a, int sms, cudaStream_t s) {
+  if (a.cols <= 8) return launch_cols<T, SPLIT, 1>(a, sms, s);
+  if (a.cols <= 16) return launch_cols<T, SPLIT, 2>(a, sms, s);
+  return launch_cols<T, SPLIT, 4>(a, sms, s);
 }
 
 int check_shape(const char *who, int64_t N, int64_t K, int group) {
@@ -454,27 +592,27 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
   a.K = (int)K;
   a.tiles_k = (int)((K + 63) / 64);
   a.groups = (int)((K + group - 1) / group);
-  a.group_tiles = group / 64;
+  a.group_tiles = std::min(group / 64, a.tiles_k);  // 0 for groups of 32
   a.out_f32 = out_f32 != 0;
+  a.group_magic = a.group_tiles > 1 ? (uint32_t)(((1ull << 32) + a.group_tiles - 1) / a.group_tiles)
+                                    : 0;
+  a.scale_bf16 = scale_dtype == B2F_BF16;
   a.x_vec = (uintptr_t)x % (4 * esize) == 0 && (rows == 1 || ldx % 4 == 0);
-  const int warps = std::min(a.tiles_k, 8);
-  a.per_warp = (a.tiles_k + warps - 1) / warps;
-  const int row_blocks = (a.N + Q4_ROWS - 1) / Q4_ROWS;
-  const int grid = std::min(row_blocks, 4 * sms);
-  const int planes = dtype == B2F_F32 ? 3 : 1, step = 32 / planes;
+  // columns of the product in one pass: up to 32, and no more than 8 blocks'
+  // shared memory holds of x (a part kept for the sums)
+  const int planes = dtype == B2F_F32 ? 3 : 1;
+  const long long fit = 8ll * (kQ4Smem - 72 * 1024) / (128ll * (a.tiles_k + 8));
+  const int step = (int)std::min<long long>(32, fit) / planes;
+  B2F_CHECK_ARG(step >= 1, "b2f_q4_matvec: %lld columns are more than shared memory holds",
+                (long long)K);
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     a.rows = (int)std::min<int64_t>(step, rows - r0);
+    a.cols = a.rows * planes;
     a.x = static_cast<const char *>(x) + r0 * ldx * esize;
     a.y = static_cast<char *>(y) + r0 * N * (out_f32 ? 4 : esize);
-    const int cols = a.rows * planes;
-    const bool z = zeros != nullptr, sb = scale_dtype == B2F_BF16;
-    int rc;
-    if (dtype == B2F_F32)
-      rc = launch_matvec_cols<__nv_bfloat16, true>(a, cols, z, sb, grid, warps, s);
-    else if (dtype == B2F_F16)
-      rc = launch_matvec_cols<__half, false>(a, cols, z, sb, grid, warps, s);
-    else
-      rc = launch_matvec_cols<__nv_bfloat16, false>(a, cols, z, sb, grid, warps, s);
+    const int rc = dtype == B2F_F32   ? launch_rows<__nv_bfloat16, true>(a, sms, s)
+                   : dtype == B2F_F16 ? launch_rows<__half, false>(a, sms, s)
+                                      : launch_rows<__nv_bfloat16, false>(a, sms, s);
     if (rc) return rc;
   }
   return B2F_OK;
