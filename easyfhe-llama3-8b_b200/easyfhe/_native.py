@@ -119,11 +119,11 @@ _SIGS = {
     "b2f_sample_secret": (_int, [_int, _u64, _int, _vp]),
     "b2f_rope": (_int, [_vp, _int, _int, _i64, _i64, _int, _int, _int, _vp, _int, _i64, _i64,
                         _vp, _dbl, _int, _vp]),
-    "b2f_q4_packed_bytes": (_size, [_i64, _i64]),
-    "b2f_q4_pack": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
+    "b2f_q4_packed_bytes": (_size, [_i64, _i64, _int, _int]),
+    "b2f_q4_pack": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _vp]),
     "b2f_q4_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp,
                                _vp]),
-    "b2f_q4_matvec": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _int, _vp, _i64, _i64, _int, _vp,
+    "b2f_q4_matvec": (_int, [_vp, _int, _i64, _i64, _vp, _int, _int, _i64, _i64, _int, _vp,
                              _int, _vp]),
     "b2f_vocab_loss_workspace": (_size, [_i64, _i64]),
     "b2f_vocab_loss": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp,

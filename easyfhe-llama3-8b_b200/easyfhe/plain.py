@@ -232,16 +232,16 @@ class Q4Weight:
     """A 4-bit weight [rows, cols] laid out for `q4_matvec` (`pack_q4`,
     `quantize_q4`): scale * (code - zero) per group of columns."""
 
-    def __init__(self, shape, group, packed, scales, scale_dtype, zeros):
+    def __init__(self, shape, group, packed, scale_dtype, zeros):
         self.shape = (int(shape[0]), int(shape[1]))
         self.group = int(group)
-        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.packed = packed  # codes, scales and zero points in records of 16 x 64
         self.scale_dtype = scale_dtype
+        self.zeros = bool(zeros)
         self.device = packed.device
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size()
-                   for t in (self.packed, self.scales, self.zeros) if t is not None)
+        return self.packed.numel()
 
 
 def _group(what: str, group: int, cols: int) -> int:
@@ -272,15 +272,13 @@ def pack_q4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
             raise ValueError(f"pack_q4: {name} above 15")
     codes, scales = codes.contiguous(), scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
-    rows16 = -(-n // 16) * 16
-    packed = torch.empty(lib.b2f_q4_packed_bytes(n, k), dtype=torch.uint8, device=dev)
-    ps = torch.empty(rows16 * groups, dtype=scales.dtype, device=dev)
-    pz = None if zeros is None else torch.empty(rows16 * groups, dtype=torch.uint8, device=dev)
+    packed = torch.empty(lib.b2f_q4_packed_bytes(n, k, int(group), int(zeros is not None)),
+                         dtype=torch.uint8, device=dev)
     with _on(dev) as stream:
         call("b2f_q4_pack", codes.data_ptr(), scales.data_ptr(),
              None if zeros is None else zeros.data_ptr(), n, k, int(group), packed.data_ptr(),
-             ps.data_ptr(), None if pz is None else pz.data_ptr(), stream)
-    return Q4Weight((n, k), group, packed, ps, scales.dtype, pz)
+             stream)
+    return Q4Weight((n, k), group, packed, scales.dtype, zeros is not None)
 
 
 def q4_codes(weight: torch.Tensor, *, group: int = 128, symmetric: bool = True,
@@ -319,8 +317,10 @@ def quantize_q4(weight: torch.Tensor, *, group: int = 128, symmetric: bool = Tru
 def q4_matvec(x: torch.Tensor, weight: Q4Weight, *,
               out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """x [..., cols] times the weight's transpose: [..., rows], up to 1024 rows
-    of x (f32, f16 or bf16; f32 keeps its 24 bits), summed in binary32.  Returns
-    x's type, or float32 with ``out_dtype=torch.float32``."""
+    of x (f32, f16 or bf16), summed in binary32.  f32 rows, and one or two rows
+    of a 16-bit type, may be taken as fixed-point numbers, off by at most 2^-30
+    of the largest of their 64 columns.  Returns x's type, or float32 with
+    ``out_dtype=torch.float32``."""
 
     if not isinstance(weight, Q4Weight):
         raise ValueError(f"q4_matvec: weight is a {type(weight).__name__}")
@@ -342,8 +342,7 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, *,
         with _on(dev) as stream:
             call("b2f_q4_matvec", x2.data_ptr(), _DTYPES[x.dtype],
                  x2.stride(0) if rows > 1 else k, rows, weight.packed.data_ptr(),
-                 weight.scales.data_ptr(), _DTYPES[weight.scale_dtype],
-                 None if weight.zeros is None else weight.zeros.data_ptr(), n, k, weight.group,
+                 _DTYPES[weight.scale_dtype], int(weight.zeros), n, k, weight.group,
                  y.data_ptr(), int(out_dtype == torch.float32), stream)
     return y
 

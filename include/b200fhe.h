@@ -495,17 +495,15 @@ int b2f_rope(const b2f_rope_heads *parts, int num_parts, int dtype, int64_t batc
              int positions64, int64_t pos_batch_stride, int64_t pos_seq_stride,
              const double *freqs, double factor, int gradient, void *stream);
 
-/* 4-bit weights [N][K] with a scale (fp16 or bf16) and optionally a zero point
+/* 4-bit weights [N][K], K up to 131072, with a scale (fp16 or bf16) and optionally a zero point
  * per row and group of `group` columns (32 or a multiple of 64; the last one
  * may be cut short): weight = scale * (code - zero), code 0..15, zero 8
- * without zero points.  Packed: b2f_q4_packed_bytes of codes, scales and zero
- * points of ceil(N / 16) * 16 rows (2 and 1 bytes each). */
-size_t b2f_q4_packed_bytes(int64_t N, int64_t K);
-/* codes [N][K] (one byte each, 0..15), scales and zeros [N][groups]; zeros and
- * packed_zeros are null for zero 8. */
+ * without zero points.  Packed: b2f_q4_packed_bytes, 32-byte aligned. */
+size_t b2f_q4_packed_bytes(int64_t N, int64_t K, int group, int zeros);
+/* codes [N][K] (one byte each, 0..15), scales and zeros [N][groups]; zeros null
+ * for zero 8. */
 int b2f_q4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, int64_t N,
-                int64_t K, int group, void *packed, void *packed_scales, void *packed_zeros,
-                void *stream);
+                int64_t K, int group, void *packed, void *stream);
 /* Codes, scales and zero points of a weight (f32, f16 or bf16, rows ld apart):
  * symmetric: scale max|w| / 7, code round(w / scale) + 8 (zeros null);
  * otherwise [min(w, 0), max(w, 0)] in 15 steps.  Finite weights. */
@@ -514,10 +512,14 @@ int b2f_q4_quantize(const void *w, int dtype, int64_t ld, int64_t N, int64_t K, 
                     uint8_t *zeros, void *stream);
 /* y[b][n] = sum_k weight[n][k] x[b][k] of up to 1024 rows of x (f32, f16 or
  * bf16, rows ldx apart), summed in binary32; y [rows][N] in x's type, or
- * binary32 with out_f32.  The weight is read once per 32 rows (10 of f32). */
+ * binary32 with out_f32.  zeros: the packed weight has zero points.  The weight is
+ * read once per 32 rows (4 of f32; fewer past about 4000 columns: what 8 blocks'
+ * shared memory holds of x).  Binary32 rows and one or two rows of a 16-bit type may
+ * be taken as fixed-point numbers, off by at most 2^-30 of the largest of their 64
+ * columns; otherwise every value of x enters exactly. */
 int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const void *packed,
-                  const void *scales, int scale_dtype, const void *zeros, int64_t N, int64_t K,
-                  int group, void *y, int out_f32, void *stream);
+                  int scale_dtype, int zeros, int64_t N, int64_t K, int group, void *y,
+                  int out_f32, void *stream);
 
 /* Softmax cross entropy of logits hidden [T][D] x weight [V][D]^T (fp16 or
  * bf16, rows ldh / ldw apart, D and both strides multiples of 8, 16-byte

@@ -42,15 +42,17 @@ def test_rope_refusals():
 
 
 def test_q4_refusals():
-    def pack(match, codes=P, scales=P, zeros=None, n=16, k=64, group=64, out=P, pz=None):
-        _refused("b2f_q4_pack", codes, scales, zeros, n, k, group, out, P, pz, None, match=match)
+    def pack(match, codes=P, scales=P, zeros=None, n=16, k=64, group=64, out=P):
+        _refused("b2f_q4_pack", codes, scales, zeros, n, k, group, out, None, match=match)
 
     pack("weight of", n=0)
+    pack("weight of", k=131073)
     pack("group of", group=96 + 1)
     pack("group of", group=48)
     pack("null", codes=None)
-    pack("null", zeros=P)  # zero points without a place for them
-    pack("misaligned", out=P + 8)
+    pack("null", out=None)
+    pack("misaligned", out=P + 16)
+    pack("misaligned", scales=P + 1)
 
     def quant(match, dtype=1, ld=64, symmetric=1, scale=3, zeros=None):
         _refused("b2f_q4_quantize", P, dtype, ld, 16, 64, 64, symmetric, scale, P, P, zeros, None,
@@ -62,8 +64,8 @@ def test_q4_refusals():
     quant("null", symmetric=0)
 
     def mv(match, x=P, dtype=3, ldx=64, rows=1, scale=3, group=64, y=P):
-        _refused("b2f_q4_matvec", x, dtype, ldx, rows, P, P, scale, None, 16, 64, group, y, 0,
-                 None, match=match)
+        _refused("b2f_q4_matvec", x, dtype, ldx, rows, P, scale, 0, 16, 64, group, y, 0, None,
+                 match=match)
 
     mv("rows", rows=1025)
     mv("dtype", dtype=0)
