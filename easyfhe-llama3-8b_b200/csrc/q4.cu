@@ -49,7 +49,7 @@
 // is refilled as soon as its tile is done).  The warps' sums of a row block meet
 // in shared memory, two buffers and one barrier per row block, and are added in
 // a fixed order.
-#include "b2f_internal.h"
+#include "plain.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -734,12 +734,13 @@ __global__ void q4_quantize_kernel(const T *__restrict__ w, long long ld, int N,
 constexpr size_t kQ4Smem = 227 * 1024;
 
 template <class T, Q4Rows HOW, int NT, bool ZERO, bool G32, bool SB>
-int launch_matvec(Q4Args a, int sms, cudaStream_t s) {
+int launch_matvec(Q4Args a, int dev, int sms, cudaStream_t s) {
   constexpr int TPW = NT > 1 || G32 ? 4 : 8;
   constexpr bool INT = HOW == Q4_DIGITS;
   auto k = q4_matvec_kernel<T, HOW, NT, TPW, ZERO, G32, SB>;
   constexpr int most = q4_max_warps(HOW);
-  B2F_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kQ4Smem));
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = allow_shared(k, (int)kQ4Smem, dev, allowed)) return rc;
   static const int regs = [&] {  // of a thread, as compiled
     cudaFuncAttributes f{};
     return cudaFuncGetAttributes(&f, k) == cudaSuccess ? (f.numRegs + 7) / 8 * 8 : 255;
@@ -786,47 +787,47 @@ int launch_matvec(Q4Args a, int sms, cudaStream_t s) {
   return B2F_OK;
 }
 template <class T, Q4Rows HOW, int NT>
-int launch_cols(const Q4Args &a, bool zero, bool g32, bool sb, int sms, cudaStream_t s) {
+int launch_cols(const Q4Args &a, bool zero, bool g32, bool sb, int dev, int sms, cudaStream_t s) {
   if (zero && g32)
-    return sb ? launch_matvec<T, HOW, NT, true, true, true>(a, sms, s)
-              : launch_matvec<T, HOW, NT, true, true, false>(a, sms, s);
+    return sb ? launch_matvec<T, HOW, NT, true, true, true>(a, dev, sms, s)
+              : launch_matvec<T, HOW, NT, true, true, false>(a, dev, sms, s);
   if (zero)
-    return sb ? launch_matvec<T, HOW, NT, true, false, true>(a, sms, s)
-              : launch_matvec<T, HOW, NT, true, false, false>(a, sms, s);
+    return sb ? launch_matvec<T, HOW, NT, true, false, true>(a, dev, sms, s)
+              : launch_matvec<T, HOW, NT, true, false, false>(a, dev, sms, s);
   if (g32)
-    return sb ? launch_matvec<T, HOW, NT, false, true, true>(a, sms, s)
-              : launch_matvec<T, HOW, NT, false, true, false>(a, sms, s);
-  return sb ? launch_matvec<T, HOW, NT, false, false, true>(a, sms, s)
-            : launch_matvec<T, HOW, NT, false, false, false>(a, sms, s);
+    return sb ? launch_matvec<T, HOW, NT, false, true, true>(a, dev, sms, s)
+              : launch_matvec<T, HOW, NT, false, true, false>(a, dev, sms, s);
+  return sb ? launch_matvec<T, HOW, NT, false, false, true>(a, dev, sms, s)
+            : launch_matvec<T, HOW, NT, false, false, false>(a, dev, sms, s);
 }
 // Binary32 rows (up to 4), or one or two rows of a 16-bit type, as digits where every
 // block has 4 (8) row blocks or more to spread their set-up over, else in their own type
 // or split.  One row of 4096 columns: binary32 12.1 against 13.8 us for 14336 weight
 // rows, 48 against 70 us for 128256, but 8.3 against 7.3 us for 4096; four binary32 rows
 // 84 against 110 us, four bf16 rows 84 against 76 us for 128256.
-int launch_rows(Q4Args a, bool zero, bool g32, bool sb, int sms, cudaStream_t s) {
+int launch_rows(Q4Args a, bool zero, bool g32, bool sb, int dev, int sms, cudaStream_t s) {
   using B = __nv_bfloat16;
   const int nt = a.rows <= 2 ? 1 : 2;
   const size_t digits = (size_t)((a.tiles_k + 7) / 8) * q4_tile_bytes(true, g32, nt, 0) + 49168;
   const int spread = (a.N + Q4_ROWS - 1) / Q4_ROWS / sms;
   if ((a.dtype == B2F_F32 ? spread >= 4 : spread >= 8 && a.rows <= 2) && digits <= kQ4Smem) {
     a.cols = 4 * a.rows;
-    return a.rows <= 2 ? launch_cols<B, Q4_DIGITS, 1>(a, zero, g32, sb, sms, s)
-                       : launch_cols<B, Q4_DIGITS, 2>(a, zero, g32, sb, sms, s);
+    return a.rows <= 2 ? launch_cols<B, Q4_DIGITS, 1>(a, zero, g32, sb, dev, sms, s)
+                       : launch_cols<B, Q4_DIGITS, 2>(a, zero, g32, sb, dev, sms, s);
   }
   if (a.dtype == B2F_F32) {
     a.cols = 3 * a.rows;
-    return a.cols <= 8 ? launch_cols<B, Q4_SPLIT, 1>(a, zero, g32, sb, sms, s)
-                       : launch_cols<B, Q4_SPLIT, 2>(a, zero, g32, sb, sms, s);
+    return a.cols <= 8 ? launch_cols<B, Q4_SPLIT, 1>(a, zero, g32, sb, dev, sms, s)
+                       : launch_cols<B, Q4_SPLIT, 2>(a, zero, g32, sb, dev, sms, s);
   }
   a.cols = a.rows;
   if (a.dtype == B2F_F16)
-    return a.cols <= 8    ? launch_cols<__half, Q4_SAME, 1>(a, zero, g32, sb, sms, s)
-           : a.cols <= 16 ? launch_cols<__half, Q4_SAME, 2>(a, zero, g32, sb, sms, s)
-                          : launch_cols<__half, Q4_SAME, 4>(a, zero, g32, sb, sms, s);
-  return a.cols <= 8    ? launch_cols<B, Q4_SAME, 1>(a, zero, g32, sb, sms, s)
-         : a.cols <= 16 ? launch_cols<B, Q4_SAME, 2>(a, zero, g32, sb, sms, s)
-                        : launch_cols<B, Q4_SAME, 4>(a, zero, g32, sb, sms, s);
+    return a.cols <= 8    ? launch_cols<__half, Q4_SAME, 1>(a, zero, g32, sb, dev, sms, s)
+           : a.cols <= 16 ? launch_cols<__half, Q4_SAME, 2>(a, zero, g32, sb, dev, sms, s)
+                          : launch_cols<__half, Q4_SAME, 4>(a, zero, g32, sb, dev, sms, s);
+  return a.cols <= 8    ? launch_cols<B, Q4_SAME, 1>(a, zero, g32, sb, dev, sms, s)
+         : a.cols <= 16 ? launch_cols<B, Q4_SAME, 2>(a, zero, g32, sb, dev, sms, s)
+                        : launch_cols<B, Q4_SAME, 4>(a, zero, g32, sb, dev, sms, s);
 }
 
 int check_shape(const char *who, int64_t N, int64_t K, int group) {
@@ -927,8 +928,7 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
                 "b2f_q4_matvec: misaligned buffer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int dev = 0, sms = 0;
-  B2F_CUDA(cudaGetDevice(&dev));
-  B2F_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (int rc = current_device(&dev, &sms)) return rc;
   Q4Args a{};
   a.packed = static_cast<const unsigned char *>(packed);
   a.ldx = ldx;
@@ -950,7 +950,8 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
     a.rows = (int)std::min<int64_t>(step, rows - r0);
     a.x = static_cast<const char *>(x) + r0 * ldx * esize;
     a.y = static_cast<char *>(y) + r0 * N * (out_f32 ? 4 : esize);
-    const int rc = launch_rows(a, zeros != 0, group == 32, scale_dtype == B2F_BF16, sms, s);
+    const int rc = launch_rows(a, zeros != 0, group == 32, scale_dtype == B2F_BF16, dev,
+                               sms, s);
     if (rc) return rc;
   }
   return B2F_OK;

@@ -34,7 +34,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "b2f_internal.h"
+#include "plain.h"
 
 namespace b2f {
 namespace {
@@ -533,16 +533,17 @@ int encode_map(CUtensorMap *m, const void *p, long long rows, long long cols, lo
 
 int sm_count(int *sms) {
   int dev = 0;
-  B2F_CUDA(cudaGetDevice(&dev));
-  B2F_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
-  return B2F_OK;
+  return current_device(&dev, sms);
 }
 
 template <class T, int EPI, bool AMN, bool BMN>
 int launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, VocabArgs a, int sms,
                 cudaStream_t s) {
   auto k = vocab_gemm_kernel<T, EPI, AMN, BMN>;
-  B2F_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)VL_SMEM));
+  static std::atomic<uint64_t> allowed{0};
+  int dev = 0;
+  if (int rc = current_device(&dev, &sms)) return rc;
+  if (int rc = allow_shared(k, (int)VL_SMEM, dev, allowed)) return rc;
   a.m_tiles = (a.M + VL_M - 1) / VL_M;
   a.n_tiles = (a.N + VL_N - 1) / VL_N;
   a.k_blocks = (a.K + VL_K - 1) / VL_K;
@@ -682,7 +683,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
 
 extern "C" {
 
-size_t b2f_vocab_loss_workspace(int64_t T, int64_t V) {
+size_t b2f_vocab_loss_workspace(int64_t T, int64_t V, int64_t D) {
   using namespace b2f;
   if (T < 1 || V < 1) return 0;
   return round256((size_t)T * 4) + round256((size_t)((V + VL_N - 1) / VL_N) * T * 8);
@@ -698,7 +699,7 @@ int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t 
   B2F_CHECK_ARG(hidden && weight && labels && loss && lse && ws, "b2f_vocab_loss: null argument");
   B2F_CHECK_ARG(((uintptr_t)hidden | (uintptr_t)weight) % 16 == 0 && (uintptr_t)ws % 256 == 0,
                 "b2f_vocab_loss: misaligned buffer (16 bytes, workspace 256)");
-  B2F_CHECK_ARG(ws_bytes >= b2f_vocab_loss_workspace(T, V),
+  B2F_CHECK_ARG(ws_bytes >= b2f_vocab_loss_workspace(T, V, D),
                 "b2f_vocab_loss: workspace too small (%zu bytes)", ws_bytes);
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;

@@ -125,7 +125,7 @@ _SIGS = {
                                _vp]),
     "b2f_q4_matvec": (_int, [_vp, _int, _i64, _i64, _vp, _int, _int, _i64, _i64, _int, _vp,
                              _int, _vp]),
-    "b2f_vocab_loss_workspace": (_size, [_i64, _i64]),
+    "b2f_vocab_loss_workspace": (_size, [_i64, _i64, _i64]),
     "b2f_vocab_loss": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp,
                               _vp, _size, _vp]),
     "b2f_vocab_loss_grad_workspace": (_size, [_i64, _i64, _i64, _int]),

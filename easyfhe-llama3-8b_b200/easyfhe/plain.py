@@ -18,59 +18,45 @@ and devices (there is no CPU fallback).
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
-from ._native import call, lib
+import struct
+
+from ._native import call, check, lib
 
 _DTYPES = {torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
+_HEADS = struct.Struct("PP6qi4x")  # b2f_rope_heads
+
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _RopeHeads(ctypes.Structure):
-    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p)] + [
-        (n, ctypes.c_int64) for n in ("in_batch", "in_seq", "in_head", "out_batch", "out_seq",
-                                      "out_head")] + [("heads", ctypes.c_int)]
+def _plain_tensor(t, index: int) -> bool:
+    """A strided CUDA tensor on device `index` that asks for no gradient."""
+
+    return isinstance(t, torch.Tensor) and t.get_device() == index and not t.is_neg() \
+        and not (t.requires_grad and torch.is_grad_enabled()) and t.layout is torch.strided
 
 
-class _on:
-    """The device of a call: current for its launches, with its raw stream."""
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self) -> int:
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-
-
-def _check(what: str, device, **tensors) -> torch.device:
-    """Every tensor a strided CUDA tensor without a gradient, on one device."""
+def _refuse(what: str, index: int | None, **tensors) -> None:
+    """Raise for the first tensor that _plain_tensor turns down."""
 
     for name, t in tensors.items():
         if t is None:
             continue
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{what}: {name} is a {type(t).__name__}, not a tensor")
+        if not t.is_cuda:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on a CUDA device")
+        if index is not None and t.get_device() != index:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected cuda:{index}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what}: {name} requires a gradient, which this call does not "
                              "record (use the explicit gradient call under torch.no_grad())")
-        if t.is_conj() or t.is_neg() or t.layout != torch.strided:
+        if not _plain_tensor(t, t.get_device()):
             raise ValueError(f"{what}: {name} is not a plain strided tensor")
-        if not t.is_cuda:
-            raise ValueError(f"{what}: {name} is on {t.device}, not on a CUDA device")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
-    return device
 
 
 # ---------------------------------------------------------------------------
@@ -154,21 +140,21 @@ class RopePlan:
                              "(2 up to the head's, heads of up to 1024)")
         if layout not in ("half", "interleaved"):
             raise ValueError(f"rope: layout {layout!r} not in ['half', 'interleaved']")
-        self.layout = layout
+        self.layout, self.interleaved = layout, int(layout == "interleaved")
         freqs, self.factor = rope_frequencies(self.rotary_dim, theta, scaling)
         dev = torch.device(device)
         if dev.type != "cuda":
             raise ValueError("rope: libb200fhe runs on CUDA devices only (no CPU fallback)")
         self.freqs = torch.tensor(freqs, dtype=torch.float64, device=dev)
-        self.device = self.freqs.device
+        self.freqs_ptr = self.freqs.data_ptr()
+        self.device, self.index = self.freqs.device, self.freqs.get_device()
 
 
-def _rope(what, q, k, positions, plan, gradient):
+def _rope_refuse(what, q, k, positions, plan):
     if not isinstance(plan, RopePlan):
         raise ValueError(f"{what}: plan is a {type(plan).__name__}")
-    dev = _check(what, plan.device, q=q, k=k, positions=positions)
-    parts = [q] if k is None else [q, k]
-    for name, t in zip("qk", parts):
+    _refuse(what, plan.index, q=q, k=k, positions=positions)
+    for name, t in (("q", q),) if k is None else (("q", q), ("k", k)):
         if t.dim() not in (3, 4) or t.shape[-1] != plan.head_dim:
             raise ValueError(f"{what}: {name} of shape {tuple(t.shape)}, expected [(batch,) seq, "
                              f"heads, {plan.head_dim}]")
@@ -179,29 +165,59 @@ def _rope(what, q, k, positions, plan, gradient):
                              f"{tuple(q.shape)}")
         if not 1 <= t.shape[-2] <= 4096:
             raise ValueError(f"{what}: {name} has {t.shape[-2]} heads (1 to 4096)")
-    batch, seq = (1, q.shape[0]) if q.dim() == 3 else (q.shape[0], q.shape[1])
     if positions.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{what}: positions are {positions.dtype} (int64 or int32)")
-    if tuple(positions.shape) not in ((seq,), (batch, seq)):
-        raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} for {batch} x "
-                         f"{seq} tokens")
-    pos_b = positions.stride(0) if positions.dim() == 2 else 0
-    parts = [t if t.stride(-1) == 1 else t.contiguous() for t in parts]
-    res = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in parts]
-    arr = (_RopeHeads * len(parts))()
-    for i, (t, o) in enumerate(zip(parts, res)):
-        ib = t.stride(0) if t.dim() == 4 else 0
-        ob = o.stride(0) if t.dim() == 4 else 0
-        arr[i] = _RopeHeads(t.data_ptr(), o.data_ptr(), ib, t.stride(-3), t.stride(-2), ob,
-                            o.stride(-3), o.stride(-2), t.shape[-2])
+    raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} for tokens of "
+                     f"{tuple(q.shape[:-2])}")
+
+
+def _rope_part(plan, t, outer):
+    """(packed b2f_rope_heads, output, input kept alive) of one tensor, None to refuse."""
+
+    shape = t.shape
+    if shape[-1] != plan.head_dim or shape[:-2] != outer or not 1 <= shape[-2] <= 4096:
+        return None
+    st = t.stride()
+    if st[-1] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    heads, dim = shape[-2], shape[-1]
+    out = t.new_empty(shape)
+    row = heads * dim
+    batch = st[0] if len(shape) == 4 else 0
+    return _HEADS.pack(t.data_ptr(), out.data_ptr(), batch, st[-3], st[-2],
+                       row * shape[-3], row, dim, heads), out, t
+
+
+def _rope(what, q, k, positions, plan, gradient):
+    if not (type(plan) is RopePlan and _plain_tensor(q, plan.index)
+            and _plain_tensor(positions, plan.index)
+            and (k is None or _plain_tensor(k, plan.index) and k.dtype is q.dtype)
+            and 3 <= q.dim() <= 4 and q.dtype in _DTYPES):
+        _rope_refuse(what, q, k, positions, plan)
+    if _current_device() != plan.index:
+        with torch.cuda.device(plan.index):
+            return _rope(what, q, k, positions, plan, gradient)
+    outer = q.shape[:-2]
+    batch, seq = outer if len(outer) == 2 else (1, outer[0])
+    pos = positions.stride()
+    wide = positions.dtype is torch.int64
+    if not (wide or positions.dtype is torch.int32) or \
+            tuple(positions.shape) not in ((seq,), (batch, seq)):
+        _rope_refuse(what, q, k, positions, plan)
+    a = _rope_part(plan, q, outer)
+    b = None if k is None else _rope_part(plan, k, outer)
+    if a is None or (b is None and k is not None):
+        _rope_refuse(what, q, k, positions, plan)
     if batch and seq:
-        with _on(dev) as stream:
-            call("b2f_rope", ctypes.addressof(arr), len(parts), _DTYPES[q.dtype], batch, seq,
-                 plan.head_dim, plan.rotary_dim, int(plan.layout == "interleaved"),
-                 positions.data_ptr(), int(positions.dtype == torch.int64), pos_b,
-                 positions.stride(-1), plan.freqs.data_ptr(), float(plan.factor),
-                 int(gradient), stream)
-    return res[0] if k is None else (res[0], res[1])
+        rc = lib.b2f_rope(a[0] if b is None else a[0] + b[0], 1 if b is None else 2,
+                          _DTYPES[q.dtype], batch, seq, plan.head_dim, plan.rotary_dim,
+                          plan.interleaved, positions.data_ptr(), wide,
+                          pos[0] if len(pos) == 2 else 0, pos[-1], plan.freqs_ptr, plan.factor,
+                          gradient, _raw_stream(plan.index))
+        if rc:
+            check(rc, what)
+    return a[1] if b is None else (a[1], b[1])
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Tensor,
@@ -213,14 +229,14 @@ def rope(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Ten
     [seq] or [batch, seq] (int64 or int32).  Returns contiguous tensors.  Angles
     are taken in binary64, products in binary32 (binary64 for f64)."""
 
-    return _rope("rope", q, k, positions, plan, False)
+    return _rope("rope", q, k, positions, plan, 0)
 
 
 def rope_grad(grad_q: torch.Tensor, grad_k: torch.Tensor | None = None, *,
               positions: torch.Tensor, plan: RopePlan):
     """The gradient of `rope`: the rotation by the negative angle."""
 
-    return _rope("rope_grad", grad_q, grad_k, positions, plan, True)
+    return _rope("rope_grad", grad_q, grad_k, positions, plan, 1)
 
 
 # ---------------------------------------------------------------------------
@@ -238,7 +254,9 @@ class Q4Weight:
         self.packed = packed  # codes, scales and zero points in records of 16 x 64
         self.scale_dtype = scale_dtype
         self.zeros = bool(zeros)
-        self.device = packed.device
+        self.device, self.index = packed.device, packed.get_device()
+        self._args = (packed.data_ptr(), _DTYPES[scale_dtype], int(self.zeros), *self.shape,
+                      self.group)
 
     def nbytes(self) -> int:
         return self.packed.numel()
@@ -257,7 +275,11 @@ def pack_q4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     (uint8, 0..15; none: 8) [rows, ceil(cols / group)] for `q4_matvec`.  Done
     once per weight: it waits for the device to check the codes."""
 
-    dev = _check("pack_q4", None, codes=codes, scales=scales, zeros=zeros)
+    _refuse("pack_q4", None, codes=codes)
+    _refuse("pack_q4", codes.get_device(), scales=scales, zeros=zeros)
+    if _current_device() != codes.get_device():
+        with torch.cuda.device(codes.get_device()):
+            return pack_q4(codes, scales, zeros, group=group)
     if codes.dim() != 2 or codes.dtype != torch.uint8 or not codes.numel():
         raise ValueError(f"pack_q4: codes of shape {tuple(codes.shape)}, {codes.dtype}")
     n, k = codes.shape
@@ -273,11 +295,10 @@ def pack_q4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     codes, scales = codes.contiguous(), scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
     packed = torch.empty(lib.b2f_q4_packed_bytes(n, k, int(group), int(zeros is not None)),
-                         dtype=torch.uint8, device=dev)
-    with _on(dev) as stream:
-        call("b2f_q4_pack", codes.data_ptr(), scales.data_ptr(),
-             None if zeros is None else zeros.data_ptr(), n, k, int(group), packed.data_ptr(),
-             stream)
+                         dtype=torch.uint8, device=codes.device)
+    call("b2f_q4_pack", codes.data_ptr(), scales.data_ptr(),
+         None if zeros is None else zeros.data_ptr(), n, k, int(group), packed.data_ptr(),
+         _raw_stream(codes.get_device()))
     return Q4Weight((n, k), group, packed, scales.dtype, zeros is not None)
 
 
@@ -287,7 +308,11 @@ def q4_codes(weight: torch.Tensor, *, group: int = 128, symmetric: bool = True,
     [rows, cols] (f32, f16 or bf16): round to nearest against the stored scale,
     max|w| / 7 of a group, or its range in 15 steps with an integer zero."""
 
-    dev = _check("q4_codes", None, weight=weight)
+    _refuse("q4_codes", None, weight=weight)
+    if _current_device() != weight.get_device():
+        with torch.cuda.device(weight.get_device()):
+            return q4_codes(weight, group=group, symmetric=symmetric, scale_dtype=scale_dtype)
+    dev = weight.device
     if weight.dim() != 2 or not weight.numel() or _DTYPES.get(weight.dtype, 0) == 0:
         raise ValueError(f"q4_codes: weight of shape {tuple(weight.shape)}, {weight.dtype}")
     if scale_dtype not in (torch.float16, torch.bfloat16):
@@ -298,10 +323,10 @@ def q4_codes(weight: torch.Tensor, *, group: int = 128, symmetric: bool = True,
     codes = torch.empty((n, k), dtype=torch.uint8, device=dev)
     scales = torch.empty((n, groups), dtype=scale_dtype, device=dev)
     zeros = None if symmetric else torch.empty((n, groups), dtype=torch.uint8, device=dev)
-    with _on(dev) as stream:
-        call("b2f_q4_quantize", w.data_ptr(), _DTYPES[w.dtype], max(w.stride(0), k), n, k,
-             int(group), int(bool(symmetric)), _DTYPES[scale_dtype], codes.data_ptr(),
-             scales.data_ptr(), None if zeros is None else zeros.data_ptr(), stream)
+    call("b2f_q4_quantize", w.data_ptr(), _DTYPES[w.dtype], max(w.stride(0), k), n, k,
+         int(group), int(bool(symmetric)), _DTYPES[scale_dtype], codes.data_ptr(),
+         scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
+         _raw_stream(weight.get_device()))
     return codes, scales, zeros
 
 
@@ -322,28 +347,37 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, *,
     of the largest of their 64 columns.  Returns x's type, or float32 with
     ``out_dtype=torch.float32``."""
 
-    if not isinstance(weight, Q4Weight):
+    if type(weight) is not Q4Weight:
         raise ValueError(f"q4_matvec: weight is a {type(weight).__name__}")
-    dev = _check("q4_matvec", weight.device, x=x)
+    if not _plain_tensor(x, weight.index):
+        _refuse("q4_matvec", weight.index, x=x)
+    if _current_device() != weight.index:
+        with torch.cuda.device(weight.index):
+            return q4_matvec(x, weight, out_dtype=out_dtype)
     n, k = weight.shape
-    if x.dim() < 1 or x.shape[-1] != k or _DTYPES.get(x.dtype, 0) == 0:
-        raise ValueError(f"q4_matvec: x of shape {tuple(x.shape)}, {x.dtype}, for {k} columns")
-    if out_dtype not in (None, x.dtype, torch.float32):
-        raise ValueError(f"q4_matvec: output in {out_dtype} for x in {x.dtype}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
+    shape, dtype = x.shape, x.dtype
+    code = _DTYPES.get(dtype, 0)
+    if not shape or shape[-1] != k or code == 0:
+        raise ValueError(f"q4_matvec: x of shape {tuple(shape)}, {dtype}, for {k} columns")
+    if out_dtype is None:
+        out_dtype = dtype
+    elif out_dtype is not dtype and out_dtype is not torch.float32:
+        raise ValueError(f"q4_matvec: output in {out_dtype} for x in {dtype}")
     rows = x.numel() // k
     if rows > 1024:
         raise ValueError(f"q4_matvec: {rows} rows (up to 1024)")
-    x2 = x if x.dim() == 2 else x.reshape(rows, k)
-    if x2.stride(1) != 1 and k > 1 or rows > 1 and x2.stride(0) < k:
-        x2 = x2.contiguous()
-    y = torch.empty((*x.shape[:-1], n), dtype=out_dtype, device=dev)
+    ld = k
+    if not x.is_contiguous():
+        x = x if x.dim() == 2 else x.reshape(rows, k)
+        if x.stride(1) != 1 and k > 1 or rows > 1 and x.stride(0) < k:
+            x = x.contiguous()
+        ld = x.stride(0) if rows > 1 else k
+    y = x.new_empty((*shape[:-1], n), dtype=out_dtype)
     if rows:
-        with _on(dev) as stream:
-            call("b2f_q4_matvec", x2.data_ptr(), _DTYPES[x.dtype],
-                 x2.stride(0) if rows > 1 else k, rows, weight.packed.data_ptr(),
-                 _DTYPES[weight.scale_dtype], int(weight.zeros), n, k, weight.group,
-                 y.data_ptr(), int(out_dtype == torch.float32), stream)
+        rc = lib.b2f_q4_matvec(x.data_ptr(), code, ld, rows, *weight._args, y.data_ptr(),
+                               out_dtype is torch.float32, _raw_stream(weight.index))
+        if rc:
+            check(rc, "q4_matvec")
     return y
 
 
@@ -352,28 +386,42 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, *,
 # ---------------------------------------------------------------------------
 
 
-def _loss_args(what, hidden, weight, labels):
-    dev = _check(what, None, hidden=hidden, weight=weight, labels=labels)
+def _rows16(m: torch.Tensor, d: int) -> torch.Tensor:
+    """m with rows as the TMA loads read them: contiguous, 16-byte aligned."""
+
+    s0, s1 = m.stride()
+    if s1 == 1 and s0 >= d and s0 % 8 == 0 and m.data_ptr() % 16 == 0:
+        return m
+    return m.clone(memory_format=torch.contiguous_format)
+
+
+def _loss_args(what, hidden, weight, labels, **more):
+    index = hidden.get_device() if isinstance(hidden, torch.Tensor) else -1
+    if index < 0 or not (_plain_tensor(hidden, index) and _plain_tensor(weight, index)
+                         and _plain_tensor(labels, index)
+                         and all(_plain_tensor(t, index) for t in more.values())):
+        _refuse(what, None, hidden=hidden)
+        _refuse(what, index, weight=weight, labels=labels, **more)
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"{what}: hidden of shape {tuple(hidden.shape)}, weight of "
                          f"{tuple(weight.shape)}")
-    if hidden.dtype not in (torch.float16, torch.bfloat16) or weight.dtype != hidden.dtype:
-        raise ValueError(f"{what}: hidden is {hidden.dtype}, weight {weight.dtype} (both "
-                         "float16 or both bfloat16)")
+    dtype = hidden.dtype
+    if not (dtype is torch.float16 or dtype is torch.bfloat16) or weight.dtype is not dtype:
+        raise ValueError(f"{what}: hidden is {dtype}, weight {weight.dtype} (both float16 or "
+                         "both bfloat16)")
     t, d = hidden.shape
-    if d % 8 or not d or not weight.shape[0]:
+    v = weight.shape[0]
+    if d % 8 or not d or not v:
         raise ValueError(f"{what}: weight of shape {tuple(weight.shape)} (a hidden size that is "
                          "a multiple of 8, at least one word)")
-    if labels.dtype != torch.int64 or tuple(labels.shape) != (t,):
+    if labels.dtype is not torch.int64 or labels.dim() != 1 or labels.shape[0] != t:
         raise ValueError(f"{what}: labels of shape {tuple(labels.shape)}, {labels.dtype}, for "
                          f"{t} tokens (int64)")
-
-    def rows(m):  # as TMA reads it: 16-byte aligned rows
-        ok = m.stride(1) == 1 and m.stride(0) >= d and m.stride(0) % 8 == 0 \
-            and m.data_ptr() % 16 == 0
-        return m if ok else m.clone(memory_format=torch.contiguous_format)
-
-    return dev, rows(hidden), rows(weight), labels.contiguous()
+    for name, x in more.items():
+        if x.dtype is not torch.float32 or x.dim() != 1 or x.shape[0] != t:
+            raise ValueError(f"{what}: {name} of shape {tuple(x.shape)}, {x.dtype}, for {t} "
+                             "tokens (float32)")
+    return index, t, v, d
 
 
 def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *,
@@ -385,17 +433,21 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
     of 8), labels int64.  A label of ignore_index gives 0; any other label
     outside the vocabulary gives NaN, as do logits that overflow."""
 
-    dev, h, w, lab = _loss_args("vocab_loss", hidden, weight, labels)
-    t, d = h.shape
-    v = w.shape[0]
-    loss = torch.empty(t, dtype=torch.float32, device=dev)
-    lse = torch.empty(t, dtype=torch.float32, device=dev)
+    index, t, v, d = _loss_args("vocab_loss", hidden, weight, labels)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return vocab_loss(hidden, weight, labels, ignore_index=ignore_index)
+    h, w, lab = _rows16(hidden, d), _rows16(weight, d), labels.contiguous()
+    loss = h.new_empty((t,), dtype=torch.float32)
+    lse = torch.empty_like(loss)
     if t:
-        ws = torch.empty(lib.b2f_vocab_loss_workspace(t, v), dtype=torch.uint8, device=dev)
-        with _on(dev) as stream:
-            call("b2f_vocab_loss", h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
-                 _DTYPES[h.dtype], t, v, d, lab.data_ptr(), int(ignore_index), loss.data_ptr(),
-                 lse.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        ws = h.new_empty((lib.b2f_vocab_loss_workspace(t, v, d),), dtype=torch.uint8)
+        rc = lib.b2f_vocab_loss(h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
+                                _DTYPES[h.dtype], t, v, d, lab.data_ptr(), int(ignore_index),
+                                loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
+                                _raw_stream(index))
+        if rc:
+            check(rc, "vocab_loss")
     return loss, lse
 
 
@@ -409,25 +461,27 @@ def vocab_loss_grad(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     The logits are computed again in pieces of the vocabulary.  Rows of ignored
     tokens contribute nothing and get zero, whatever they hold."""
 
-    what = "vocab_loss_grad"
-    dev, h, w, lab = _loss_args(what, hidden, weight, labels)
-    _check(what, dev, lse=lse, grad_loss=grad_loss)
-    t, d = h.shape
-    v = w.shape[0]
-    for name, x in (("lse", lse), ("grad_loss", grad_loss)):
-        if x.dtype != torch.float32 or tuple(x.shape) != (t,):
-            raise ValueError(f"{what}: {name} of shape {tuple(x.shape)}, {x.dtype}, for {t} "
-                             "tokens (float32)")
+    index, t, v, d = _loss_args("vocab_loss_grad", hidden, weight, labels, lse=lse,
+                                grad_loss=grad_loss)
     if not (need_hidden or need_weight):
-        raise ValueError(f"{what}: no gradient asked for")
+        raise ValueError("vocab_loss_grad: no gradient asked for")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return vocab_loss_grad(hidden, weight, labels, lse, grad_loss,
+                                   ignore_index=ignore_index, need_hidden=need_hidden,
+                                   need_weight=need_weight)
+    h, w, lab = _rows16(hidden, d), _rows16(weight, d), labels.contiguous()
     lse, g = lse.contiguous(), grad_loss.contiguous()
-    dh = torch.empty((t, d), dtype=h.dtype, device=dev) if need_hidden else None
-    dw = torch.empty((v, d), dtype=w.dtype, device=dev) if need_weight else None
-    with _on(dev) as stream:
-        ws = torch.empty(max(lib.b2f_vocab_loss_grad_workspace(t, v, d, int(need_hidden)), 16),
-                         dtype=torch.uint8, device=dev)
-        call("b2f_vocab_loss_grad", h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
-             _DTYPES[h.dtype], t, v, d, lab.data_ptr(), int(ignore_index), lse.data_ptr(),
-             g.data_ptr(), None if dh is None else dh.data_ptr(),
-             None if dw is None else dw.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    dh = h.new_empty((t, d)) if need_hidden else None
+    dw = w.new_empty((v, d)) if need_weight else None
+    ws = h.new_empty((max(lib.b2f_vocab_loss_grad_workspace(t, v, d, bool(need_hidden)), 16),),
+                     dtype=torch.uint8)
+    rc = lib.b2f_vocab_loss_grad(h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
+                                 _DTYPES[h.dtype], t, v, d, lab.data_ptr(), int(ignore_index),
+                                 lse.data_ptr(), g.data_ptr(),
+                                 None if dh is None else dh.data_ptr(),
+                                 None if dw is None else dw.data_ptr(), ws.data_ptr(),
+                                 ws.numel(), _raw_stream(index))
+    if rc:
+        check(rc, "vocab_loss_grad")
     return dh, dw

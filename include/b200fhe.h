@@ -526,7 +526,7 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
  * aligned) against labels [T], without the logits being kept: lse[t] = log sum_v
  * exp z_tv, loss[t] = lse[t] - z_{t, label}; 0 where the label is `ignore`, NaN
  * where it is any other value outside [0, V).  Workspace 256-byte aligned. */
-size_t b2f_vocab_loss_workspace(int64_t T, int64_t V);
+size_t b2f_vocab_loss_workspace(int64_t T, int64_t V, int64_t D);
 int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int dtype,
                    int64_t T, int64_t V, int64_t D, const int64_t *labels, int64_t ignore,
                    float *loss, float *lse, void *ws, size_t ws_bytes, void *stream);

@@ -10,8 +10,6 @@ pass through are equal."""
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 
@@ -178,8 +176,8 @@ def test_in_place_through_the_c_abi():
         q = _x(9, 3, 96, dtype=dtype)
         pos = torch.arange(9, device="cuda")
         want = plain.rope(q, positions=pos, plan=plan)
-        part = plain._RopeHeads(q.data_ptr(), q.data_ptr(), 0, 288, 96, 0, 288, 96, 3)
-        _native.call("b2f_rope", ctypes.addressof(part), 1, plain._DTYPES[dtype], 1, 9, 96, 64,
+        part = plain._HEADS.pack(q.data_ptr(), q.data_ptr(), 0, 288, 96, 0, 288, 96, 3)
+        _native.call("b2f_rope", part, 1, plain._DTYPES[dtype], 1, 9, 96, 64,
                      int(layout == "interleaved"), pos.data_ptr(), 1, 0, 1,
                      plan.freqs.data_ptr(), plan.factor, 0,
                      torch.cuda.current_stream().cuda_stream)

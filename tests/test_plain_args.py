@@ -3,7 +3,6 @@ arguments before anything touches a device, and the host-side plans theirs."""
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import pytest
@@ -21,10 +20,11 @@ def _refused(name, *args, match, kind=ValueError):
 def test_rope_refusals():
     from easyfhe import plain
 
-    part = plain._RopeHeads(P, P, 0, 64, 64, 0, 64, 64, 1)
+    def heads(where, count):
+        return plain._HEADS.pack(where, P, 0, 64, 64, 0, 64, 64, count)
 
-    def bad(match, p=part, parts=1, dtype=3, batch=1, seq=1, dim=64, rotary=64, pos=P, freqs=P):
-        _refused("b2f_rope", ctypes.addressof(p) if p else None, parts, dtype, batch, seq, dim,
+    def bad(match, p=heads(P, 1), parts=1, dtype=3, batch=1, seq=1, dim=64, rotary=64, pos=P, freqs=P):
+        _refused("b2f_rope", p, parts, dtype, batch, seq, dim,
                  rotary, 0, pos, 1, 0, 1, freqs, 1.0, 0, None, match=match)
 
     bad("one or two", p=None)
@@ -37,8 +37,8 @@ def test_rope_refusals():
     bad("tokens", batch=1 << 20, seq=1 << 20)
     bad("null", pos=None)
     bad("null", freqs=None)
-    bad("misaligned", p=plain._RopeHeads(P + 1, P, 0, 64, 64, 0, 64, 64, 1))
-    bad("heads", p=plain._RopeHeads(P, P, 0, 64, 64, 0, 64, 64, 0))
+    bad("misaligned", p=heads(P + 1, 1))
+    bad("heads", p=heads(P, 0))
 
 
 def test_q4_refusals():
