@@ -9,19 +9,24 @@
 // Three matrix products on tcgen05 (bf16 or fp16 operands, binary32
 // accumulators in tensor memory), one kernel template:
 //   logits   A = h (K-major), B = W (K-major); the epilogue either reduces the
-//            tile's 256 columns to (max, sum of exp) per token, or turns
-//            them into dz and stores that in the operand type;
+//            tile's columns to (max, sum of exp) per token, or turns them into
+//            dz and stores that in the operand type;
 //   dh       A = dz (K-major), B = W read along its rows (N-major);
 //   dW       A = dz^T (M-major), B = h (N-major).
 // The gradient walks the vocabulary in pieces whose dz fits a workspace: the
 // logits of a piece are computed again, become dz at once, and both products
-// consume it.
+// consume it.  Ignored tokens are left out: the counted ones are gathered first,
+// and the tiles are counted off from their number on the device.
 //
 // One block per SM: warp 0 loads tiles by TMA (128-byte swizzle) into a ring of
-// stages, warp 1 issues the MMAs (128 x 256 x 16), warps 2-5 read the
-// accumulators; two accumulators in tensor memory let the epilogue of a tile
-// run under the products of the next.  Every wait is bounded: a wait that
-// runs out ends the block and is counted (b2f_vocab_loss_wait_errors).
+// stages, warp 1 issues the MMAs, warps 2-9 read the accumulators; two
+// accumulators in tensor memory let the epilogue of a tile run under the products
+// of the next.  Either a block computes tiles of 128 x 128, or (more than 128
+// tokens) two blocks of a cluster tiles of 256 x 256 (cta_group::2), each loading
+// half of both operands: 64 bytes of shared memory per 256 x 256 x 1 instead of 96
+// for a 128 x 256 tile of one SM.  Outputs leave through shared memory as TMA
+// stores.  Every wait is bounded: a wait that runs out ends the block and is counted
+// (b2f_vocab_loss_wait_errors).
 //
 // dz is rounded once to the operand type before its two products: relative to
 // each dz at most half a step of the type, the size of the rounding of the
@@ -39,16 +44,18 @@
 namespace b2f {
 namespace {
 
-constexpr int VL_M = 128;       // rows of a tile (TMEM lanes)
-constexpr int VL_N = 256;       // columns of a tile
+constexpr int VL_M = 128;       // rows of a block's part of a tile (TMEM lanes)
+constexpr int VL_N = 128;       // columns of B that a block loads
 constexpr int VL_K = 64;        // K step: one 128-byte swizzle row
-constexpr int VL_STAGES = 4;
+constexpr int VL_STAGES = 5;
 constexpr int VL_A_BYTES = VL_M * VL_K * 2;
-constexpr int VL_B_BYTES = VL_N * VL_K * 2;
-constexpr int VL_STAGE = VL_A_BYTES + VL_B_BYTES;
-constexpr int VL_THREADS = 192;
-constexpr int VL_BARRIERS = 256;  // bytes in front of the stages' alignment slack
-constexpr size_t VL_SMEM = (size_t)VL_STAGES * VL_STAGE + VL_BARRIERS + 1024;
+constexpr int VL_STAGE = VL_A_BYTES + VL_N * VL_K * 2;
+constexpr int VL_EPI_WARPS = 8;
+constexpr int VL_THREADS = 32 * (2 + VL_EPI_WARPS);
+constexpr int VL_SLAB = 4096;   // 32 rows of 128 bytes that a warp stores at once
+constexpr int VL_BARRIERS = 256;
+constexpr size_t VL_SMEM = 1024 + (size_t)VL_STAGES * VL_STAGE + VL_EPI_WARPS * 2 * VL_SLAB +
+                           VL_BARRIERS;
 constexpr int VL_WAIT_LIMIT = 1 << 23;  // polls (each may suspend the thread for a while)
 static_assert(VL_SMEM <= 227 * 1024, "stages exceed shared memory");
 
@@ -56,25 +63,43 @@ __device__ int g_vocab_wait_errors;
 
 enum Epilogue { EPI_STATS, EPI_DZ, EPI_PARTIAL, EPI_OUT };
 
+// Tokens as the products see them: `rows` of the workspace, the counted ones first.
+struct Counted {
+  const int *count;          // how many; null: all of them
+  const long long *labels;   // of the counted tokens
+  const float *lse, *grad;
+  const uint32_t *grad_max;  // bits of max |g| (fp16)
+};
+
 struct VocabArgs {
-  int M, N, K;          // the product's sizes
-  int m_tiles, n_tiles, splits, k_blocks, split_blocks;  // K blocks in all, of a split
-  int n_first;          // first row of B's outer coordinate (logits: first word of the piece)
-  int k_first;          // dh: first word of the piece (row of W)
-  // logits
-  const long long *labels;
+  int M, N, K;        // the product's sizes (M or K in tokens: at most that many)
+  int splits;         // of K
+  int n_first;        // logits: first word of the piece
+  int k_first;        // dh: first word of the piece (row of W)
+  int m_first;        // dW: first word of the piece (row of dW)
+  int tokens_in_k;    // K counts tokens (dW), else M does
+  Counted tok;
   long long ignore;
   int vocab;
-  float2 *part;         // [n_tiles][M] (max, sum)
-  float *label_logit;   // [M]
-  const float *lse, *grad;
-  const uint32_t *grad_max;  // bits of max |g| (fp16 only)
-  void *out;            // dz, dh or dW
-  long long ld_out;
-  // dh partial sums
-  float *partial;       // [splits][M][N]
-  int accumulate;
+  float2 *part;       // [slots][M] (max, sum)
+  float *label_logit; // [M]
+  int accumulate;     // dh: add to the partial sums
 };
+
+// The tiles of a product, as every warp counts them off.
+struct Tiles {
+  int m_tiles, n_tiles, k_blocks, split_blocks, total;
+};
+template <int CG>
+__host__ __device__ inline Tiles tiles_of(const VocabArgs &a, int M, int K) {
+  Tiles t;
+  t.m_tiles = (M + CG * VL_M - 1) / (CG * VL_M);
+  t.n_tiles = (a.N + CG * VL_N - 1) / (CG * VL_N);
+  t.k_blocks = (K + VL_K - 1) / VL_K;
+  t.split_blocks = (t.k_blocks + a.splits - 1) / a.splits;
+  t.total = t.m_tiles * t.n_tiles * a.splits;
+  return t;
+}
 
 __device__ __forceinline__ uint32_t sptr(const void *p) {
   return (uint32_t)__cvta_generic_to_shared(p);
@@ -86,9 +111,6 @@ __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(sptr(bar)),
                "r"(bytes)
                : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(sptr(bar)) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
   uint32_t done;
@@ -111,28 +133,100 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
   atomicAdd(&g_vocab_wait_errors, 1);
   return false;
 }
-__device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *map, int x, int y,
-                                       uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3}], [%4];\n" ::"r"(sptr(dst)),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(sptr(bar))
-      : "memory");
+// address of a shared-memory object in another block of the cluster
+__device__ __forceinline__ uint32_t in_block(const void *p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(sptr(p)), "r"(rank));
+  return a;
 }
+__device__ __forceinline__ void bar_arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// tile load; bar: shared::cluster address, of the pair's first block for CG 2
+template <int CG>
+__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int y,
+                                         uint32_t bar) {
+  if (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];\n" ::"r"(sptr(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%2, %3}], [%4];\n" ::"r"(sptr(dst)),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y,
+                                          const void *src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n"
+               ::"l"((uint64_t)map), "r"(x), "r"(y), "r"(sptr(src))
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, int x, int y, int z,
+                                             const void *src, bool add) {
+  if (add)
+    asm volatile(
+        "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group "
+        "[%0, {%1, %2, %3}], [%4];\n" ::"l"((uint64_t)map), "r"(x), "r"(y), "r"(z),
+        "r"(sptr(src))
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n"
+        ::"l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(sptr(src))
+        : "memory");
+}
+__device__ __forceinline__ void store_commit() {
+  asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+// all but the last `n` stores have read their shared memory
+template <int n>
+__device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(n) : "memory");
+}
+__device__ __forceinline__ void store_wait() {
+  asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+}
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
+// the MMAs issued so far arrive on the barrier when done (CG 2: in both blocks)
+template <int CG>
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
-          sptr(bar))
-      : "memory");
+  if (CG == 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
+            sptr(bar))
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;\n" ::"r"(sptr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -190,202 +284,151 @@ __device__ __forceinline__ float dz_scale(const uint32_t *grad_max) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <class T, int EPI>
-__device__ __forceinline__ void epilogue_tile(const VocabArgs &a, uint32_t tmem, int m0, int n0,
-                                              int split, int row) {
-  const int t = m0 + row;
-  const bool live = t < a.M;
-  if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
-    const long long label = live ? a.labels[t] : a.ignore;
-    // column of the label in this tile
-    const long long at = label - a.n_first - n0;
-    const int hit = at >= 0 && at < VL_N ? (int)at : -1;
-    const int cols = min(VL_N, a.N - n0);
-    if constexpr (EPI == EPI_STATS) {
-      float mx = -INFINITY, sum = 0.0f;
-      for (int c = 0; c < VL_N; c += 32) {
-        if (c >= cols) break;
-        __syncwarp();  // the tensor-memory load takes the whole warp
-        float v[32];
-        tmem_ld32(tmem + c, v);
-        if (c + 32 > cols)
+// 2^x, values below 2^-126 as zero
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// element h (-1: none) of v
+__device__ __forceinline__ float pick(const float (&v)[32], int h) {
+  float z = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j >= cols) v[j] = -INFINITY;
-        float m2 = mx;
+  for (int j = 0; j < 32; ++j)
+    if (j == h) z = v[j];
+  return z;
+}
+// running (max, sum of 2^((v - max) log2 e)) joined with another; an empty one is
+// (-inf, 0) and must not make inf - inf of its own
+__device__ __forceinline__ void join(float &m, float &s, float m1, float s1) {
+  const float m2 = fmaxf(m, m1), base = m2 == -INFINITY ? 0.0f : m2;
+  s = s * ex2((m - base) * kLog2e) + s1 * ex2((m1 - base) * kLog2e);
+  m = m2;
+}
+
+// 32 columns of this warp's 32 rows into a slab (rows of 128 bytes, 16-byte chunks
+// XORed with the row as TMA's 128-byte swizzle has them): as 64 bytes of 16-bit values
+// (half 0 or 1 of the row) or 128 bytes of binary32.
+template <class T>
+__device__ __forceinline__ void put_half(unsigned char *slab, int lane, int half,
+                                         const float (&v)[32]) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) m2 = fmaxf(m2, v[j]);
-        // an empty maximum must not make inf - inf of its own
-        const float base = m2 == -INFINITY ? 0.0f : m2;
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s += exp2f((v[j] - base) * kLog2e);
-        sum = sum * exp2f((mx - base) * kLog2e) + s;
-        mx = m2;
-        if ((hit >> 5) == (c >> 5) && hit >= 0) {
-          float z = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j == hit) z = v[j];
-          if (live) a.label_logit[t] = z;
-        }
-      }
-      if (live) a.part[(long long)(n0 / VL_N) * a.M + t] = make_float2(mx, sum);
-    } else {
-      const bool counted = live && label != a.ignore;
-      const bool valid = label >= 0 && label < a.vocab;
-      float g = counted ? a.grad[t] : 0.0f;
-      if (counted && !valid) g = NAN;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value)
-        g *= dz_scale(a.grad_max);
-      const float lse = live ? a.lse[t] : 0.0f;
-      T *out = static_cast<T *>(a.out) + (long long)t * a.ld_out + n0;
-      for (int c = 0; c < VL_N; c += 32) {
-        if (c >= cols) break;
-        __syncwarp();  // the tensor-memory load takes the whole warp
-        float v[32];
-        tmem_ld32(tmem + c, v);
-        if (!live) continue;
-        const int h = (hit >> 5) == (c >> 5) && hit >= 0 ? hit - c : -1;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float x = v[j] - lse;
-          float p = exp2f(x * kLog2e);
-          if (j == h) p = expm1f(x);
-          v[j] = counted ? g * p : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 32; j += 8)
-          if (c + j < cols) {
-            uint4 w;
-            w.x = pack2<T>(v[j], v[j + 1]);
-            w.y = pack2<T>(v[j + 2], v[j + 3]);
-            w.z = pack2<T>(v[j + 4], v[j + 5]);
-            w.w = pack2<T>(v[j + 6], v[j + 7]);
-            *reinterpret_cast<uint4 *>(out + c + j) = w;
-          }
-      }
-    }
-  } else {
-    float scale = 1.0f;
-    if constexpr (std::is_same<T, __half>::value) scale = 1.0f / dz_scale(a.grad_max);
-    const int cols = min(VL_N, a.N - n0);
-    for (int c = 0; c < VL_N; c += 32) {
-      if (c >= cols) break;
-      __syncwarp();
-      float v[32];
-      tmem_ld32(tmem + c, v);
-      if (!live) continue;
-      if constexpr (EPI == EPI_PARTIAL) {
-        float *out = a.partial + ((long long)split * a.M + t) * a.N + n0 + c;
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          if (c + j < cols) {
-            float4 w = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            if (a.accumulate) {
-              const float4 o = *reinterpret_cast<const float4 *>(out + j);
-              w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
-            }
-            *reinterpret_cast<float4 *>(out + j) = w;
-          }
-      } else {
-        T *out = static_cast<T *>(a.out) + (long long)t * a.ld_out + n0 + c;
-#pragma unroll
-        for (int j = 0; j < 32; j += 8)
-          if (c + j < cols) {
-            uint4 w;
-            w.x = pack2<T>(v[j] * scale, v[j + 1] * scale);
-            w.y = pack2<T>(v[j + 2] * scale, v[j + 3] * scale);
-            w.z = pack2<T>(v[j + 4] * scale, v[j + 5] * scale);
-            w.w = pack2<T>(v[j + 6] * scale, v[j + 7] * scale);
-            *reinterpret_cast<uint4 *>(out + j) = w;
-          }
-      }
-    }
+  for (int c = 0; c < 4; ++c) {
+    uint4 w;
+    w.x = pack2<T>(v[8 * c], v[8 * c + 1]);
+    w.y = pack2<T>(v[8 * c + 2], v[8 * c + 3]);
+    w.z = pack2<T>(v[8 * c + 4], v[8 * c + 5]);
+    w.w = pack2<T>(v[8 * c + 6], v[8 * c + 7]);
+    *reinterpret_cast<uint4 *>(slab + lane * 128 + (((4 * half + c) ^ (lane & 7)) << 4)) = w;
   }
+}
+__device__ __forceinline__ void put_floats(unsigned char *slab, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<float4 *>(slab + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
 }
 
 // D[M][N] = sum_k A[m][k] B[n][k] per tile and split, handed to the epilogue.
 // AMN / BMN: the operand lies in memory with M (N) contiguous, so a stage of it
-// is blocks of 64 M (N) values x 64 K rows instead of rows of 64 K values.
-template <class T, int EPI, bool AMN, bool BMN>
+// is blocks of 64 M (N) values x 64 K rows instead of rows of 64 K values.  CG: blocks
+// that share a tile.
+template <class T, int EPI, bool AMN, bool BMN, int CG>
 __global__ void __launch_bounds__(VL_THREADS, 1)
     vocab_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
-                      const __grid_constant__ CUtensorMap map_b, const VocabArgs a) {
+                      const __grid_constant__ CUtensorMap map_b,
+                      const __grid_constant__ CUtensorMap map_out, const VocabArgs a) {
+  constexpr int TILE_M = CG * VL_M, TILE_N = CG * VL_N;
   extern __shared__ unsigned char vl_raw[];
-  unsigned char *base = vl_raw + VL_BARRIERS;
-  base += (1024 - (sptr(base) & 1023)) & 1023;
-  uint64_t *full = reinterpret_cast<uint64_t *>(vl_raw + ((16 - (sptr(vl_raw) & 15)) & 15));
+  unsigned char *base = vl_raw + ((1024 - (sptr(vl_raw) & 1023)) & 1023);
+  unsigned char *slabs = base + VL_STAGES * VL_STAGE;
+  uint64_t *full = reinterpret_cast<uint64_t *>(slabs + VL_EPI_WARPS * 2 * VL_SLAB);
   uint64_t *empty = full + VL_STAGES, *acc_full = empty + VL_STAGES, *acc_empty = acc_full + 2;
   uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(acc_empty + 2);
   volatile int *lost = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank = 0;
+  if (CG > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
   if (threadIdx.x == 0) {
     for (int s = 0; s < VL_STAGES; ++s) bar_init(full + s, 1), bar_init(empty + s, 1);
-    for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, 128);
+    for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, CG * VL_EPI_WARPS);
     *lost = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
-                     sptr(tmem_ptr)),
-                 "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+    if (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                       sptr(tmem_ptr)),
+                   "r"(2 * TILE_N));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
+                       sptr(tmem_ptr)),
+                   "r"(2 * TILE_N));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
+    }
   }
   fence_before();
   __syncthreads();
+  if (CG > 1) cluster_meet();
   fence_after();
   const uint32_t tmem = *tmem_ptr;
-  const int tiles = a.m_tiles * a.n_tiles * a.splits;
+  int M = a.M, K = a.K;
+  if (a.tok.count) (a.tokens_in_k ? K : M) = *a.tok.count;
+  const Tiles ts = tiles_of<CG>(a, M, K);
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const bool sums = ts.k_blocks > 0;  // no counted token: dW is zero without a product
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && sums) {
       int it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        const int mt = tile % a.m_tiles, r = tile / a.m_tiles;
-        const int nt = r % a.n_tiles, split = r / a.n_tiles;
-        const int kb0 = split * a.split_blocks, kb1 = min(kb0 + a.split_blocks, a.k_blocks);
+      for (int tile = first; tile < ts.total && ok; tile += step) {
+        const int mt = tile % ts.m_tiles, r = tile / ts.m_tiles;
+        const int nt = r % ts.n_tiles, split = r / ts.n_tiles;
+        const int kb0 = split * ts.split_blocks, kb1 = min(kb0 + ts.split_blocks, ts.k_blocks);
+        const int m0 = mt * TILE_M + rank * VL_M, n0 = nt * TILE_N + rank * VL_N;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % VL_STAGES;
           if (it >= VL_STAGES &&
               !(ok = bar_wait(empty + s, ((it / VL_STAGES) - 1) & 1, lost)))
             break;
           unsigned char *sa = base + s * VL_STAGE, *sb = sa + VL_A_BYTES;
-          bar_expect(full + s, VL_STAGE);
+          if (rank == 0) bar_expect(full + s, CG * VL_STAGE);
+          const uint32_t bar = CG == 1 ? sptr(full + s) : in_block(full + s, 0);
           if (AMN) {
 #pragma unroll
             for (int i = 0; i < VL_M / 64; ++i)
-              tma_2d(sa + i * 8192, &map_a, mt * VL_M + i * 64, kb * VL_K, full + s);
+              tma_load<CG>(sa + i * 8192, &map_a, m0 + i * 64, kb * VL_K, bar);
           } else {
-            tma_2d(sa, &map_a, kb * VL_K, mt * VL_M, full + s);
+            tma_load<CG>(sa, &map_a, kb * VL_K, m0, bar);
           }
           if (BMN) {
 #pragma unroll
             for (int i = 0; i < VL_N / 64; ++i)
-              tma_2d(sb + i * 8192, &map_b, nt * VL_N + i * 64, a.k_first + kb * VL_K, full + s);
+              tma_load<CG>(sb + i * 8192, &map_b, n0 + i * 64, a.k_first + kb * VL_K, bar);
           } else {
-            tma_2d(sb, &map_b, kb * VL_K, a.n_first + nt * VL_N, full + s);
+            tma_load<CG>(sb, &map_b, kb * VL_K, a.n_first + n0, bar);
           }
         }
       }
-      if (!ok)  // let the loads in flight land before the block ends
+      if (!ok && rank == 0)  // let the loads in flight land before the block ends
         for (int i = max(0, it - VL_STAGES); i < it; ++i)
           for (int p = 0; p < VL_WAIT_LIMIT && !bar_try(full + i % VL_STAGES, (i / VL_STAGES) & 1);
                ++p) {
           }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0 && sums) {
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)AMN << 15) |
-                                 ((uint32_t)BMN << 16) | ((uint32_t)(VL_N >> 3) << 17) |
-                                 ((uint32_t)(VL_M >> 4) << 24);
+                                 ((uint32_t)BMN << 16) | ((uint32_t)(TILE_N >> 3) << 17) |
+                                 ((uint32_t)(TILE_M >> 4) << 24);
       int it = 0, n = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
-        const int split = tile / (a.m_tiles * a.n_tiles);
-        const int kb0 = split * a.split_blocks, kb1 = min(kb0 + a.split_blocks, a.k_blocks);
+      for (int tile = first; tile < ts.total && ok; tile += step, ++n) {
+        const int split = tile / (ts.m_tiles * ts.n_tiles);
+        const int kb0 = split * ts.split_blocks, kb1 = min(kb0 + ts.split_blocks, ts.k_blocks);
         const int buf = n & 1;
         if (n >= 2 && !(ok = bar_wait(acc_empty + buf, ((n >> 1) - 1) & 1, lost))) break;
         fence_after();
@@ -396,95 +439,289 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
           const uint32_t sa = sptr(base + s * VL_STAGE), sb = sa + VL_A_BYTES;
 #pragma unroll
           for (int k = 0; k < VL_K / 16; ++k)
-            mma_f16(tmem + buf * VL_N, swizzled_desc(sa + k * (AMN ? 2048 : 32), 8192),
-                    swizzled_desc(sb + k * (BMN ? 2048 : 32), 8192), idesc,
-                    kb > kb0 || k > 0);
-          mma_commit(empty + s);
+            mma_f16<CG>(tmem + buf * TILE_N, swizzled_desc(sa + k * (AMN ? 2048 : 32), 8192),
+                        swizzled_desc(sb + k * (BMN ? 2048 : 32), 8192), idesc,
+                        kb > kb0 || k > 0);
+          mma_commit<CG>(empty + s);
         }
-        if (ok) mma_commit(acc_full + buf);
+        if (ok) mma_commit<CG>(acc_full + buf);
       }
     }
   } else {
-    const int row = (warp & 3) * 32 + lane;
-    int n = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-      const int mt = tile % a.m_tiles, r = tile / a.m_tiles;
-      const int nt = r % a.n_tiles, split = r / a.n_tiles;
+    // warps of lane quarter (warp & 3); two of them share a quarter's columns
+    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
+    constexpr int COLS = TILE_N / 2;
+    unsigned char *slab = slabs + (warp - 2) * 2 * VL_SLAB;
+    int used = 0, n = 0;
+    float scale = 1.0f;
+    if constexpr (std::is_same<T, __half>::value && EPI != EPI_STATS)
+      scale = dz_scale(a.tok.grad_max);
+    if (EPI != EPI_DZ) scale = 1.0f / scale;
+    float run_max = -INFINITY, run_sum = 0.0f;  // stats of one row over a block's tiles
+    for (int tile = first; tile < ts.total; tile += step, ++n) {
+      const int mt = tile % ts.m_tiles, r = tile / ts.m_tiles;
+      const int nt = r % ts.n_tiles, split = r / ts.n_tiles;
       const int buf = n & 1;
-      const bool ok = bar_wait(acc_full + buf, (n >> 1) & 1, lost);
-      if (!__all_sync(~0u, ok)) break;
-      fence_after();
-      epilogue_tile<T, EPI>(a, tmem + buf * VL_N + ((uint32_t)((warp & 3) * 32) << 16),
-                            mt * VL_M, nt * VL_N, split, row);
+      if (sums) {
+        const bool ok = bar_wait(acc_full + buf, (n >> 1) & 1, lost);
+        if (!__all_sync(~0u, ok)) break;
+        fence_after();
+      }
+      const uint32_t acc =
+          tmem + buf * TILE_N + half * COLS + ((uint32_t)(quarter * 32) << 16);
+      const int m0 = mt * TILE_M + rank * VL_M, n0 = nt * TILE_N + half * COLS;
+      const int t = m0 + row, cols = a.N - n0;  // columns of the product from n0 on
+      // the next free slab, read out by its earlier store
+      auto next_slab = [&]() {
+        if (lane == 0) store_wait_read<1>();
+        __syncwarp();
+        return slab + (used++ & 1) * VL_SLAB;
+      };
+      auto filled = [&]() {
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+      };
+      if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
+        const bool live = t < M;
+        const long long label = live ? a.tok.labels[t] : a.ignore;
+        const long long at = label - a.n_first - n0;  // the label's column here
+        const int hit = at >= 0 && at < COLS && at < cols ? (int)at : -1;
+        float g = 0.0f, lse = 0.0f;
+        if (EPI == EPI_DZ && live && label != a.ignore) {
+          g = a.tok.grad[t] * scale;
+          lse = a.tok.lse[t];
+          if (label < 0 || label >= a.vocab) g = NAN;
+        }
+        float mx = -INFINITY, sum = 0.0f;
+        for (int c = 0; c < COLS; c += EPI == EPI_STATS ? 32 : 64) {
+          if (c >= cols) break;
+          if constexpr (EPI == EPI_STATS) {
+            __syncwarp();  // the tensor-memory load takes the whole warp
+            float v[32];
+            tmem_ld32(acc + c, v);
+            if (c + 32 > cols)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c + j >= cols) v[j] = -INFINITY;
+            float m2 = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) m2 = fmaxf(m2, v[j]);
+            const float bs = m2 == -INFINITY ? 0.0f : m2;
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s += ex2((v[j] - bs) * kLog2e);
+            join(mx, sum, m2, s);
+            if (hit >= c && hit < c + 32) a.label_logit[t] = pick(v, hit - c);
+          } else {
+            unsigned char *sl = next_slab();
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              __syncwarp();
+              float v[32];
+              tmem_ld32(acc + c + 32 * q, v);
+              const int h = hit - c - 32 * q;
+              const float own = h >= 0 && h < 32 ? g * expm1f(pick(v, h) - lse) : 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float p = ex2((v[j] - lse) * kLog2e);
+                v[j] = g == 0.0f ? 0.0f : g * p;  // 0 too where the logits are not finite
+                if (j == h) v[j] = own;
+              }
+              put_half<T>(sl, lane, q, v);
+            }
+            filled();
+            if (lane == 0 && m0 + quarter * 32 < a.M) {
+              tma_store(&map_out, n0 + c, m0 + quarter * 32, sl);
+              store_commit();
+            }
+          }
+        }
+        if constexpr (EPI == EPI_STATS) {
+          // with one tile of tokens a block's tiles all hold the same rows: one entry
+          // per block; else one per tile
+          const bool one = a.M <= TILE_M;  // as the host counts the entries
+          if (one) {
+            join(run_max, run_sum, mx, sum);
+            mx = run_max, sum = run_sum;
+          }
+          if (live && (!one || tile + step >= ts.total))
+            a.part[(long long)((one ? first : nt) * 2 + half) * a.M + t] = make_float2(mx, sum);
+        }
+      } else if constexpr (EPI == EPI_PARTIAL) {
+        for (int c = 0; c < COLS && c < cols; c += 32) {
+          unsigned char *sl = next_slab();
+          float v[32];
+          tmem_ld32(acc + c, v);
+          put_floats(sl, lane, v);
+          filled();
+          if (lane == 0 && m0 + quarter * 32 < a.M) {
+            tma_store_3d(&map_out, n0 + c, m0 + quarter * 32, split, sl, a.accumulate);
+            store_commit();
+          }
+        }
+      } else {
+        for (int c = 0; c < COLS && c < cols; c += 64) {
+          unsigned char *sl = next_slab();
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float v[32];
+            if (sums) {
+              tmem_ld32(acc + c + 32 * q, v);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+            }
+            if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= scale;
+            }
+            put_half<T>(sl, lane, q, v);
+          }
+          filled();
+          if (lane == 0 && m0 + quarter * 32 < a.M) {
+            tma_store(&map_out, n0 + c, a.m_first + m0 + quarter * 32, sl);
+            store_commit();
+          }
+        }
+      }
       fence_before();
-      bar_arrive(acc_empty + buf);
+      __syncwarp();
+      if (lane == 0 && sums) bar_arrive_at(in_block(acc_empty + buf, 0));
     }
+    if (EPI != EPI_STATS && lane == 0) store_wait();
   }
   __syncwarp();
   fence_before();
   __syncthreads();
+  if (CG > 1) cluster_meet();
   fence_after();
-  if (warp == 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
-                 "r"(512));
+  if (warp == 1) {
+    if (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
+                   "r"(2 * TILE_N));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
+                   "r"(2 * TILE_N));
+  }
 }
 
-// Joins the tiles' (max, sum): block (32 tokens, 16 slices of the tiles).
+// Joins the tiles' (max, sum): block (8 tokens, 64 slices of the entries).  Ignored
+// tokens get 0 and 0.  place: where a token's entries are (null: at its own number).
 __global__ void __launch_bounds__(512)
     vocab_join_kernel(const float2 *__restrict__ part, const float *__restrict__ label_logit,
                       const long long *__restrict__ labels, long long ignore, int vocab,
-                      int T, int n_tiles, float *__restrict__ loss, float *__restrict__ lse) {
-  __shared__ float2 sm[16][33];
-  const int t = blockIdx.x * 32 + threadIdx.x;
+                      const int *__restrict__ place, int T, int slots, float *__restrict__ loss,
+                      float *__restrict__ lse) {
+  __shared__ float2 sm[64][9];
+  const int t = blockIdx.x * 8 + threadIdx.x;
+  const bool live = t < T && labels[t] != ignore;
+  const int at = live ? (place ? place[t] : t) : 0;
   float m = -INFINITY, s = 0.0f;
-  auto join = [&](float2 p) {
-    const float m2 = fmaxf(m, p.x), base = m2 == -INFINITY ? 0.0f : m2;
-    s = s * exp2f((m - base) * kLog2e) + p.y * exp2f((p.x - base) * kLog2e);
-    m = m2;
-  };
-  if (t < T)
-    for (int n = threadIdx.y; n < n_tiles; n += 16) join(part[(long long)n * T + t]);
+  if (live) {
+#pragma unroll 8
+    for (int n = threadIdx.y; n < slots; n += 64) {
+      const float2 p = part[(long long)n * T + at];
+      join(m, s, p.x, p.y);
+    }
+  }
   sm[threadIdx.y][threadIdx.x] = make_float2(m, s);
   __syncthreads();
+  if (threadIdx.y >= 8) return;
+  for (int y = threadIdx.y + 8; y < 64; y += 8) join(m, s, sm[y][threadIdx.x].x, sm[y][threadIdx.x].y);
+  sm[threadIdx.y][threadIdx.x] = make_float2(m, s);
+  asm volatile("bar.sync 1, 64;\n" ::: "memory");
   if (threadIdx.y || t >= T) return;
-  m = -INFINITY, s = 0.0f;
-  for (int y = 0; y < 16; ++y) join(sm[y][threadIdx.x]);
-  const long long label = labels[t];
+  for (int y = 1; y < 8; ++y) join(m, s, sm[y][threadIdx.x].x, sm[y][threadIdx.x].y);
   const float ls = logf(s);
-  lse[t] = m + ls;
+  lse[t] = live ? m + ls : 0.0f;
   float l = 0.0f;
-  if (label != ignore) l = label >= 0 && label < vocab ? (m - label_logit[t]) + ls : NAN;
+  if (live) l = labels[t] >= 0 && labels[t] < vocab ? (m - label_logit[at]) + ls : NAN;
   loss[t] = l;
 }
 
-// Hidden states with the rows of ignored tokens set to zero (whatever lies
-// there, infinities and NaN included, must not reach dW) and max |g|.
-template <class T>
-__global__ void __launch_bounds__(128)
-    vocab_mask_kernel(const T *__restrict__ h, long long ldh, int D,
-                      const long long *__restrict__ labels, long long ignore,
-                      const float *__restrict__ grad, T *__restrict__ out,
-                      uint32_t *__restrict__ grad_max) {
-  const long long t = blockIdx.x;
-  const bool counted = labels[t] != ignore;
-  const uint4 *in = reinterpret_cast<const uint4 *>(h + t * ldh);
-  uint4 *o = reinterpret_cast<uint4 *>(out + t * D);
-  for (int i = threadIdx.x; i < D / 8; i += 128)
-    o[i] = counted ? in[i] : make_uint4(0, 0, 0, 0);
-  if (grad_max && threadIdx.x == 0 && counted)
-    atomicMax(grad_max, __float_as_uint(fabsf(grad[t])));
+// Where each counted token goes (-1: ignored), how many there are, max |g|.
+__global__ void __launch_bounds__(1024)
+    vocab_count_kernel(const long long *__restrict__ labels, long long ignore,
+                       const float *__restrict__ grad, int T, int *__restrict__ place,
+                       int *__restrict__ count, uint32_t *__restrict__ grad_max) {
+  __shared__ int sums[32];
+  __shared__ uint32_t tops[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int before = 0;
+  uint32_t top = 0;
+  for (int t0 = 0; t0 < T; t0 += 1024) {
+    const int t = t0 + threadIdx.x;
+    const bool in = t < T && labels[t] != ignore;
+    const uint32_t mask = __ballot_sync(~0u, in);
+    if (in && grad) top = max(top, __float_as_uint(fabsf(grad[t])));
+    if (lane == 0) sums[warp] = __popc(mask);
+    __syncthreads();
+    int v = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(~0u, v, o);
+      if (lane >= o) v += u;
+    }
+    const int mine = before + __shfl_sync(~0u, v, warp) - __popc(mask) + __popc(mask & ((1u << lane) - 1));
+    before += __shfl_sync(~0u, v, 31);
+    if (t < T) place[t] = in ? mine : -1;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) top = max(top, tops[w]);
+    *count = before;
+    if (grad_max) *grad_max = top;
+  }
 }
 
-// Sum of the splits' dh, in order, rounded once.
+// The counted tokens' rows, labels, lse and g, packed; up to 63 zero rows behind them
+// fill the last K block of dW.
 template <class T>
-__global__ void vocab_sum_kernel(const float4 *__restrict__ partial, int splits, long long n4,
-                                 const uint32_t *__restrict__ grad_max, uint2 *__restrict__ out) {
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n4) return;
-  float4 v = partial[i];
-  for (int s = 1; s < splits; ++s) {
-    const float4 w = partial[(long long)s * n4 + i];
-    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+__global__ void __launch_bounds__(128)
+    vocab_gather_kernel(const T *__restrict__ h, long long ldh, int D, int tokens,
+                        const int *__restrict__ place, const int *__restrict__ count,
+                        const long long *__restrict__ labels, const float *__restrict__ lse,
+                        const float *__restrict__ grad, T *__restrict__ out,
+                        long long *__restrict__ out_labels, float *__restrict__ out_lse,
+                        float *__restrict__ out_grad) {
+  const int t = blockIdx.x, p = place[t];
+  if (p >= 0) {
+    const uint4 *in = reinterpret_cast<const uint4 *>(h + t * ldh);
+    uint4 *o = reinterpret_cast<uint4 *>(out + (long long)p * D);
+    for (int i = threadIdx.x; i < D / 8; i += 128) o[i] = in[i];
+    if (threadIdx.x == 0) {
+      out_labels[p] = labels[t];
+      if (lse) out_lse[p] = lse[t], out_grad[p] = grad[t];
+    }
+  }
+  const int zero = *count + t;
+  if (t < 63 && zero < tokens) {
+    uint4 *o = reinterpret_cast<uint4 *>(out + (long long)zero * D);
+    for (int i = threadIdx.x; i < D / 8; i += 128) o[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Sum of the splits' dh, in order, rounded once; zero rows for ignored tokens.
+template <class T>
+__global__ void __launch_bounds__(256)
+    vocab_sum_kernel(const float4 *__restrict__ partial, int splits, int tokens, int d4,
+                     const int *__restrict__ place, const uint32_t *__restrict__ grad_max,
+                     uint2 *__restrict__ out) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)tokens * d4) return;
+  const int t = (int)(i / d4), c = (int)(i - (long long)t * d4), p = place[t];
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (p >= 0) {
+    const float4 *from = partial + (long long)p * d4 + c;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) {
+      const float4 w = from[(long long)s * tokens * d4];
+      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    }
   }
   float scale = 1.0f;
   if constexpr (std::is_same<T, __half>::value) scale = 1.0f / dz_scale(grad_max);
@@ -505,55 +742,78 @@ TensorMapEncoder map_encoder() {
   return fn;
 }
 
-// matrix [rows][cols] of 16-bit values, rows ld apart, in boxes of 64 columns
-template <class T>
-int encode_map(CUtensorMap *m, const void *p, long long rows, long long cols, long long ld,
-               int box_rows) {
+int encode(CUtensorMap *m, CUtensorMapDataType type, int rank, const void *p,
+           const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
   const TensorMapEncoder enc = map_encoder();
   if (!enc) {
     set_error("the driver has no cuTensorMapEncodeTiled");
     return B2F_ERR_UNSUPPORTED;
   }
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, es[2] = {1, 1};
-  const CUresult r =
-      enc(m,
-          std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-          2, const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(m, type, rank, const_cast<void *>(p), dims, strides, box, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
-    set_error("tensor map of %lld x %lld (rows %lld apart): error %d", rows, cols, ld, (int)r);
+    set_error("tensor map of %llu x %llu: error %d", (unsigned long long)dims[1],
+              (unsigned long long)dims[0], (int)r);
     return B2F_ERR_CUDA;
   }
   return B2F_OK;
 }
-
-int sm_count(int *sms) {
-  int dev = 0;
-  return current_device(&dev, sms);
+// matrix [rows][cols] of 16-bit values, rows ld apart, in boxes of 64 columns
+template <class T>
+int encode_map(CUtensorMap *m, const void *p, long long rows, long long cols, long long ld,
+               int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  return encode(m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                2, p, dims, strides, box);
+}
+// [splits][rows][cols] of binary32 in boxes of 32 x 32
+int encode_partial(CUtensorMap *m, const float *p, long long splits, long long rows,
+                   long long cols) {
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)splits};
+  const cuuint64_t strides[2] = {(cuuint64_t)cols * 4, (cuuint64_t)(rows * cols) * 4};
+  const cuuint32_t box[3] = {32, 32, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p, dims, strides, box);
 }
 
-template <class T, int EPI, bool AMN, bool BMN>
-int launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, VocabArgs a, int sms,
-                cudaStream_t s) {
-  auto k = vocab_gemm_kernel<T, EPI, AMN, BMN>;
+// Blocks that share a tile: two from 129 tokens on.  With up to 128 tokens W's bytes
+// bound every product and half of a 256-row tile would be empty.
+int blocks_per_tile(int64_t T) { return T > VL_M ? 2 : 1; }
+
+template <class T, int EPI, bool AMN, bool BMN, int CG>
+int launch_tiles(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo,
+                 const VocabArgs &a, int dev, int sms, cudaStream_t s) {
+  auto k = vocab_gemm_kernel<T, EPI, AMN, BMN, CG>;
   static std::atomic<uint64_t> allowed{0};
-  int dev = 0;
-  if (int rc = current_device(&dev, &sms)) return rc;
   if (int rc = allow_shared(k, (int)VL_SMEM, dev, allowed)) return rc;
-  a.m_tiles = (a.M + VL_M - 1) / VL_M;
-  a.n_tiles = (a.N + VL_N - 1) / VL_N;
-  a.k_blocks = (a.K + VL_K - 1) / VL_K;
-  a.split_blocks = (a.k_blocks + a.splits - 1) / a.splits;
-  a.splits = (a.k_blocks + a.split_blocks - 1) / a.split_blocks;  // none empty
-  const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
-  B2F_CHECK_ARG(tiles < (1ll << 31), "b2f_vocab_loss: %lld tiles", tiles);
-  k<<<(unsigned)std::min<long long>(tiles, sms), VL_THREADS, VL_SMEM, s>>>(ma, mb, a);
+  const int64_t m_tiles = (a.M + CG * VL_M - 1) / (CG * VL_M);
+  const int64_t n_tiles = (a.N + CG * VL_N - 1) / (CG * VL_N);
+  B2F_CHECK_ARG(m_tiles * n_tiles * a.splits < (1ll << 31), "b2f_vocab_loss: too many tiles");
+  const int tiles = (int)(m_tiles * n_tiles * a.splits);
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(CG * std::min(tiles, sms / CG));
+  c.blockDim = dim3(VL_THREADS);
+  c.dynamicSmemBytes = VL_SMEM;
+  c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = CG > 1 ? 1 : 0;
+  B2F_CUDA(cudaLaunchKernelEx(&c, k, ma, mb, mo, a));
   B2F_LAUNCHED("vocab_gemm_kernel");
   return B2F_OK;
+}
+template <class T, int EPI, bool AMN, bool BMN>
+int launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo,
+                const VocabArgs &a, int group, int dev, int sms, cudaStream_t s) {
+  return group == 2 ? launch_tiles<T, EPI, AMN, BMN, 2>(ma, mb, mo, a, dev, sms, s)
+                    : launch_tiles<T, EPI, AMN, BMN, 1>(ma, mb, mo, a, dev, sms, s);
 }
 
 struct Shape {
@@ -563,31 +823,88 @@ struct Shape {
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// The counted tokens' place in a workspace.
+struct CountedSpace {
+  size_t place, count, gmax, labels, lse, grad, rows, end;
+};
+CountedSpace counted_space(int64_t T, int64_t D, bool grad) {
+  CountedSpace c{};
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t at = off;
+    off += round256(n);
+    return at;
+  };
+  c.place = take(T * 4), c.count = take(4), c.gmax = take(4), c.labels = take(T * 8);
+  c.lse = take(grad ? T * 4 : 0), c.grad = take(grad ? T * 4 : 0);
+  c.rows = take((size_t)T * D * 2);
+  c.end = off;
+  return c;
+}
+template <class T>
+int gather_counted(const void *h, const Shape &z, const long long *labels, long long ignore,
+                   const float *lse, const float *grad, char *ws, const CountedSpace &c,
+                   Counted *tok, cudaStream_t s) {
+  int *place = reinterpret_cast<int *>(ws + c.place), *count = reinterpret_cast<int *>(ws + c.count);
+  auto *gmax = reinterpret_cast<uint32_t *>(ws + c.gmax);
+  auto *lab = reinterpret_cast<long long *>(ws + c.labels);
+  float *l = reinterpret_cast<float *>(ws + c.lse), *g = reinterpret_cast<float *>(ws + c.grad);
+  vocab_count_kernel<<<1, 1024, 0, s>>>(labels, ignore, grad, z.T, place, count, gmax);
+  B2F_LAUNCHED("vocab_count_kernel");
+  vocab_gather_kernel<T><<<z.T, 128, 0, s>>>(static_cast<const T *>(h), z.ldh, z.D, z.T, place,
+                                             count, labels, lse, grad,
+                                             reinterpret_cast<T *>(ws + c.rows), lab, l, g);
+  B2F_LAUNCHED("vocab_gather_kernel");
+  *tok = Counted{count, lab, l, g, gmax};
+  return B2F_OK;
+}
+
+// The forward pass gathers the counted tokens too from 1024 tokens on, where a product
+// over the ignored ones costs more than two more launches.
+bool forward_gathers(int64_t T) { return T >= 1024; }
+int64_t forward_slots(int64_t T, int64_t V, int sms) {
+  const int64_t group = blocks_per_tile(T), tiles = (V + group * VL_N - 1) / (group * VL_N);
+  // entries of blocks where one tile holds all tokens, else of tiles
+  return 2 * (T <= group * VL_M ? std::min<int64_t>(tiles, sms / group) : tiles);
+}
+
 // How the gradient is cut: words of a piece, splits of dh's sum over a piece.
 struct Plan {
   int piece, pieces, splits;
-  size_t hc, dz, partial, gmax, total;
+  CountedSpace c;
+  size_t dz, partial, total;
 };
 constexpr size_t kDzBytes = 256ull << 20;
 
 Plan grad_plan(int64_t T, int64_t V, int64_t D, bool need_h, int sms) {
   Plan p{};
-  int64_t words = (int64_t)(kDzBytes / 2 / (size_t)T) / VL_N * VL_N;
-  words = std::max<int64_t>(words, VL_N);
+  constexpr int unit = 2 * VL_N;
+  int64_t words = (int64_t)(kDzBytes / 2 / (size_t)T) / unit * unit;
+  words = std::max<int64_t>(words, unit);
   p.pieces = (int)((V + words - 1) / words);
-  p.piece = (int)(((V + p.pieces - 1) / p.pieces + VL_N - 1) / VL_N * VL_N);
+  p.piece = (int)(((V + p.pieces - 1) / p.pieces + unit - 1) / unit * unit);
   p.pieces = (int)((V + p.piece - 1) / p.piece);
-  const int64_t tiles = ((T + VL_M - 1) / VL_M) * ((D + VL_N - 1) / VL_N);
+  // splits of a piece's words in dh = dz W: the number (with at least 4 K blocks
+  // each) whose rounds over the SMs leave the least idle, 6 K blocks counted for a
+  // tile's store; at most 256 MB of partial sums beyond the first
+  const int64_t group = blocks_per_tile(T), slots = sms / group;
+  const int64_t tiles = ((T + group * VL_M - 1) / (group * VL_M)) *
+                        ((D + group * VL_N - 1) / (group * VL_N));
   const int64_t kb = (std::min<int64_t>(p.piece, V) + VL_K - 1) / VL_K;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 4));
-  const int64_t per = (kb + p.splits - 1) / p.splits;
-  p.splits = (int)((kb + per - 1) / per);  // every split of the first piece has work
-  size_t off = 0;
-  p.hc = off, off += round256((size_t)T * D * 2);
+  int64_t best = 0;
+  p.splits = 1;
+  for (int64_t n = 1; n <= slots && n <= std::max<int64_t>(1, kb / 4); ++n) {
+    if (n > 1 && (size_t)(n - 1) * T * D * 4 > (256ull << 20)) break;
+    const int64_t per = (kb + n - 1) / n;
+    if ((kb + per - 1) / per != n) continue;  // a split without work
+    const int64_t cost = ((tiles * n + slots - 1) / slots) * (per + 6);
+    if (!best || cost < best) best = cost, p.splits = (int)n;
+  }
+  p.c = counted_space(T, D, true);
+  size_t off = p.c.end;
   p.dz = off, off += round256((size_t)T * p.piece * 2);
   p.partial = off;
   if (need_h) off += round256((size_t)p.splits * T * D * 4);
-  p.gmax = off, off += 256;
   p.total = off;
   return p;
 }
@@ -607,18 +924,35 @@ int check_shape(const char *who, int dtype, int64_t T, int64_t V, int64_t D, int
 
 template <class T>
 int forward(const void *h, const void *w, const Shape &z, const long long *labels,
-            long long ignore, float *loss, float *lse, void *ws, int sms, cudaStream_t s) {
-  CUtensorMap ma, mb;
-  if (int rc = encode_map<T>(&ma, h, z.T, z.D, z.ldh, VL_M)) return rc;
-  if (int rc = encode_map<T>(&mb, w, z.V, z.D, z.ldw, VL_N)) return rc;
+            long long ignore, float *loss, float *lse, char *ws, int dev, int sms,
+            cudaStream_t s) {
   VocabArgs a{};
   a.M = z.T, a.N = z.V, a.K = z.D, a.splits = 1;
-  a.labels = labels, a.ignore = ignore, a.vocab = z.V;
-  a.label_logit = static_cast<float *>(ws);
-  a.part = reinterpret_cast<float2 *>(static_cast<char *>(ws) + round256((size_t)z.T * 4));
-  if (int rc = launch_gemm<T, EPI_STATS, false, false>(ma, mb, a, sms, s)) return rc;
-  vocab_join_kernel<<<(z.T + 31) / 32, dim3(32, 16), 0, s>>>(
-      a.part, a.label_logit, labels, ignore, z.V, z.T, (z.V + VL_N - 1) / VL_N, loss, lse);
+  a.ignore = ignore, a.vocab = z.V;
+  a.tok.labels = labels;
+  const int group = blocks_per_tile(z.T);
+  const int64_t slots = forward_slots(z.T, z.V, sms);
+  a.label_logit = reinterpret_cast<float *>(ws);
+  size_t off = round256((size_t)z.T * 4);
+  a.part = reinterpret_cast<float2 *>(ws + off);
+  off += round256((size_t)slots * z.T * 8);
+  const int *place = nullptr;
+  long long ldh = z.ldh;
+  if (forward_gathers(z.T)) {
+    const CountedSpace c = counted_space(z.T, z.D, false);
+    if (int rc = gather_counted<T>(h, z, labels, ignore, nullptr, nullptr, ws + off, c, &a.tok, s))
+      return rc;
+    h = ws + off + c.rows;
+    ldh = z.D;
+    place = reinterpret_cast<int *>(ws + off + c.place);
+  }
+  CUtensorMap ma, mb;
+  if (int rc = encode_map<T>(&ma, h, z.T, z.D, ldh, VL_M)) return rc;
+  if (int rc = encode_map<T>(&mb, w, z.V, z.D, z.ldw, VL_N)) return rc;
+  if (int rc = launch_gemm<T, EPI_STATS, false, false>(ma, mb, ma, a, group, dev, sms, s))
+    return rc;
+  vocab_join_kernel<<<(z.T + 7) / 8, dim3(8, 64), 0, s>>>(a.part, a.label_logit, labels, ignore,
+                                                          z.V, place, z.T, (int)slots, loss, lse);
   B2F_LAUNCHED("vocab_join_kernel");
   return B2F_OK;
 }
@@ -626,53 +960,55 @@ int forward(const void *h, const void *w, const Shape &z, const long long *label
 template <class T>
 int backward(const void *h, const void *w, const Shape &z, const long long *labels,
              long long ignore, const float *lse, const float *grad, void *dh, void *dw,
-             const Plan &p, char *ws, int sms, cudaStream_t s) {
-  T *hc = reinterpret_cast<T *>(ws + p.hc), *dz = reinterpret_cast<T *>(ws + p.dz);
+             const Plan &p, char *ws, int dev, int sms, cudaStream_t s) {
+  T *hc = reinterpret_cast<T *>(ws + p.c.rows), *dz = reinterpret_cast<T *>(ws + p.dz);
   float *partial = reinterpret_cast<float *>(ws + p.partial);
-  uint32_t *gmax = nullptr;
-  if (std::is_same<T, __half>::value) {
-    gmax = reinterpret_cast<uint32_t *>(ws + p.gmax);
-    B2F_CUDA(cudaMemsetAsync(gmax, 0, 4, s));
-  }
-  vocab_mask_kernel<T><<<z.T, 128, 0, s>>>(static_cast<const T *>(h), z.ldh, z.D, labels, ignore,
-                                           grad, hc, gmax);
-  B2F_LAUNCHED("vocab_mask_kernel");
-  CUtensorMap h_k, h_n, w_k, w_n, dz_k, dz_m;
+  Counted tok;
+  if (int rc = gather_counted<T>(h, z, labels, ignore, lse, grad, ws, p.c, &tok, s)) return rc;
+  const int group = blocks_per_tile(z.T);
+  CUtensorMap h_k, h_n, w_k, w_n, dz_k, dz_m, dz_out, sums, dw_out;
   if (int rc = encode_map<T>(&h_k, hc, z.T, z.D, z.D, VL_M)) return rc;
   if (int rc = encode_map<T>(&w_k, w, z.V, z.D, z.ldw, VL_N)) return rc;
   if (int rc = encode_map<T>(&h_n, hc, z.T, z.D, z.D, VL_K)) return rc;
   if (int rc = encode_map<T>(&w_n, w, z.V, z.D, z.ldw, VL_K)) return rc;
+  if (dh)
+    if (int rc = encode_partial(&sums, partial, p.splits, z.T, z.D)) return rc;
+  if (dw)
+    if (int rc = encode_map<T>(&dw_out, dw, z.V, z.D, z.D, 32)) return rc;
   for (int i = 0; i < p.pieces; ++i) {
     const int v0 = i * p.piece, words = std::min(p.piece, z.V - v0);
     VocabArgs a{};
     a.M = z.T, a.N = words, a.K = z.D, a.splits = 1;
     a.n_first = v0;
-    a.labels = labels, a.ignore = ignore, a.vocab = z.V;
-    a.lse = lse, a.grad = grad, a.grad_max = gmax;
-    a.out = dz, a.ld_out = p.piece;
-    if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, a, sms, s)) return rc;
+    a.tok = tok, a.ignore = ignore, a.vocab = z.V;
+    if (int rc = encode_map<T>(&dz_out, dz, z.T, words, p.piece, 32)) return rc;
+    if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, dz_out, a, group, dev, sms, s))
+      return rc;
     if (dh) {
       if (int rc = encode_map<T>(&dz_k, dz, z.T, words, p.piece, VL_M)) return rc;
       VocabArgs b{};
       b.M = z.T, b.N = z.D, b.K = words, b.splits = p.splits;
       b.k_first = v0;
-      b.partial = partial, b.accumulate = i > 0;
-      if (int rc = launch_gemm<T, EPI_PARTIAL, false, true>(dz_k, w_n, b, sms, s)) return rc;
+      b.tok = tok;
+      b.accumulate = i > 0;
+      if (int rc = launch_gemm<T, EPI_PARTIAL, false, true>(dz_k, w_n, sums, b, group, dev, sms, s))
+        return rc;
     }
     if (dw) {
       if (int rc = encode_map<T>(&dz_m, dz, z.T, words, p.piece, VL_K)) return rc;
       VocabArgs b{};
       b.M = words, b.N = z.D, b.K = z.T, b.splits = 1;
-      b.grad_max = gmax;
-      b.out = static_cast<T *>(dw) + (long long)v0 * z.D, b.ld_out = z.D;
-      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, b, sms, s)) return rc;
+      b.m_first = v0;
+      b.tok = tok, b.tokens_in_k = 1;
+      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, dw_out, b, group, dev, sms, s))
+        return rc;
     }
   }
   if (dh) {
     const long long n4 = (long long)z.T * z.D / 4;
     vocab_sum_kernel<T><<<(unsigned)((n4 + 255) / 256), 256, 0, s>>>(
-        reinterpret_cast<const float4 *>(partial), p.splits, n4, gmax,
-        static_cast<uint2 *>(dh));
+        reinterpret_cast<const float4 *>(partial), p.splits, z.T, z.D / 4,
+        reinterpret_cast<const int *>(ws + p.c.place), tok.grad_max, static_cast<uint2 *>(dh));
     B2F_LAUNCHED("vocab_sum_kernel");
   }
   return B2F_OK;
@@ -685,8 +1021,10 @@ extern "C" {
 
 size_t b2f_vocab_loss_workspace(int64_t T, int64_t V, int64_t D) {
   using namespace b2f;
-  if (T < 1 || V < 1) return 0;
-  return round256((size_t)T * 4) + round256((size_t)((V + VL_N - 1) / VL_N) * T * 8);
+  int dev = 0, sms = 0;
+  if (T < 1 || V < 1 || D < 1 || current_device(&dev, &sms)) return 0;
+  return round256((size_t)T * 4) + round256((size_t)forward_slots(T, V, sms) * T * 8) +
+         (forward_gathers(T) ? counted_space(T, D, false).end : 0);
 }
 
 int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int dtype,
@@ -699,22 +1037,23 @@ int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t 
   B2F_CHECK_ARG(hidden && weight && labels && loss && lse && ws, "b2f_vocab_loss: null argument");
   B2F_CHECK_ARG(((uintptr_t)hidden | (uintptr_t)weight) % 16 == 0 && (uintptr_t)ws % 256 == 0,
                 "b2f_vocab_loss: misaligned buffer (16 bytes, workspace 256)");
+  int dev = 0, sms = 0;
+  if (int rc = current_device(&dev, &sms)) return rc;
   B2F_CHECK_ARG(ws_bytes >= b2f_vocab_loss_workspace(T, V, D),
                 "b2f_vocab_loss: workspace too small (%zu bytes)", ws_bytes);
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
+  char *wsp = static_cast<char *>(ws);
   const Shape z{(int)T, (int)D, (int)V, ldh, ldw};
   auto *lab = reinterpret_cast<const long long *>(labels);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == B2F_F16
-             ? forward<__half>(hidden, weight, z, lab, ignore, loss, lse, ws, sms, s)
-             : forward<__nv_bfloat16>(hidden, weight, z, lab, ignore, loss, lse, ws, sms, s);
+             ? forward<__half>(hidden, weight, z, lab, ignore, loss, lse, wsp, dev, sms, s)
+             : forward<__nv_bfloat16>(hidden, weight, z, lab, ignore, loss, lse, wsp, dev, sms, s);
 }
 
 size_t b2f_vocab_loss_grad_workspace(int64_t T, int64_t V, int64_t D, int need_hidden) {
   using namespace b2f;
-  int sms = 0;
-  if (T < 1 || V < 1 || D < 1 || sm_count(&sms)) return 0;
+  int dev = 0, sms = 0;
+  if (T < 1 || V < 1 || D < 1 || current_device(&dev, &sms)) return 0;
   return grad_plan(T, V, D, need_hidden != 0, sms).total;
 }
 
@@ -737,8 +1076,8 @@ int b2f_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int
   B2F_CHECK_ARG(((uintptr_t)hidden | (uintptr_t)weight | (uintptr_t)grad_hidden |
                  (uintptr_t)grad_weight) % 16 == 0 && (uintptr_t)ws % 256 == 0,
                 "b2f_vocab_loss_grad: misaligned buffer (16 bytes, workspace 256)");
-  int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
+  int dev = 0, sms = 0;
+  if (int rc = current_device(&dev, &sms)) return rc;
   const Plan p = grad_plan(T, V, D, grad_hidden != nullptr, sms);
   B2F_CHECK_ARG(ws_bytes >= p.total, "b2f_vocab_loss_grad: workspace too small (%zu of %zu bytes)",
                 ws_bytes, p.total);
@@ -747,9 +1086,9 @@ int b2f_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int
   char *w = static_cast<char *>(ws);
   return dtype == B2F_F16
              ? backward<__half>(hidden, weight, z, lab, ignore, lse, grad_loss, grad_hidden,
-                                grad_weight, p, w, sms, s)
+                                grad_weight, p, w, dev, sms, s)
              : backward<__nv_bfloat16>(hidden, weight, z, lab, ignore, lse, grad_loss,
-                                       grad_hidden, grad_weight, p, w, sms, s);
+                                       grad_hidden, grad_weight, p, w, dev, sms, s);
 }
 
 int b2f_vocab_loss_wait_errors(void) {

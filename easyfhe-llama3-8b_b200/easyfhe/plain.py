@@ -430,8 +430,8 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
     without the logits: (loss [tokens], lse [tokens]) in float32.
 
     hidden [tokens, D], weight [words, D] (both f16 or both bf16, D a multiple
-    of 8), labels int64.  A label of ignore_index gives 0; any other label
-    outside the vocabulary gives NaN, as do logits that overflow."""
+    of 8), labels int64.  A label of ignore_index gives 0 for both; any other
+    label outside the vocabulary gives a loss of NaN, as do logits that overflow."""
 
     index, t, v, d = _loss_args("vocab_loss", hidden, weight, labels)
     if _current_device() != index:

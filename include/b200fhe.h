@@ -524,8 +524,9 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
 /* Softmax cross entropy of logits hidden [T][D] x weight [V][D]^T (fp16 or
  * bf16, rows ldh / ldw apart, D and both strides multiples of 8, 16-byte
  * aligned) against labels [T], without the logits being kept: lse[t] = log sum_v
- * exp z_tv, loss[t] = lse[t] - z_{t, label}; 0 where the label is `ignore`, NaN
- * where it is any other value outside [0, V).  Workspace 256-byte aligned. */
+ * exp z_tv, loss[t] = lse[t] - z_{t, label}; both 0 where the label is `ignore`,
+ * loss NaN where it is any other value outside [0, V).  Workspace 256-byte
+ * aligned, its query for the current device. */
 size_t b2f_vocab_loss_workspace(int64_t T, int64_t V, int64_t D);
 int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int dtype,
                    int64_t T, int64_t V, int64_t D, const int64_t *labels, int64_t ignore,
