@@ -19,12 +19,12 @@
 // and the tiles are counted off from their number on the device.
 //
 // One block per SM: warp 0 loads tiles by TMA (128-byte swizzle) into a ring of
-// stages, warp 1 issues the MMAs, warps 2-9 read the accumulators; two
+// stages, warp 1 issues the MMAs, 8 or 16 more read the accumulators; two
 // accumulators in tensor memory let the epilogue of a tile run under the products
-// of the next.  Either a block computes tiles of 128 x 128, or (more than 128
-// tokens) two blocks of a cluster tiles of 256 x 256 (cta_group::2), each loading
-// half of both operands: 64 bytes of shared memory per 256 x 256 x 1 instead of 96
-// for a 128 x 256 tile of one SM.  Outputs leave through shared memory as TMA
+// of the next.  Either a block computes tiles of 128 x 256, or (dW, and the others
+// with more than 128 tokens) two blocks of a cluster tiles of 256 x 256
+// (cta_group::2), each loading half of both operands: 32 KB a K step instead of 48
+// for as much of the product.  Outputs leave through shared memory as TMA
 // stores.  Every wait is bounded: a wait that runs out ends the block and is counted
 // (b2f_vocab_loss_wait_errors).
 //
@@ -45,19 +45,29 @@ namespace b2f {
 namespace {
 
 constexpr int VL_M = 128;       // rows of a block's part of a tile (TMEM lanes)
-constexpr int VL_N = 128;       // columns of B that a block loads
+constexpr int VL_N = 256;       // columns of a tile
 constexpr int VL_K = 64;        // K step: one 128-byte swizzle row
-constexpr int VL_STAGES = 5;
-constexpr int VL_A_BYTES = VL_M * VL_K * 2;
-constexpr int VL_STAGE = VL_A_BYTES + VL_N * VL_K * 2;
-constexpr int VL_EPI_WARPS = 8;
-constexpr int VL_THREADS = 32 * (2 + VL_EPI_WARPS);
 constexpr int VL_SLAB = 4096;   // 32 rows of 128 bytes that a warp stores at once
-constexpr int VL_BARRIERS = 256;
-constexpr size_t VL_SMEM = 1024 + (size_t)VL_STAGES * VL_STAGE + VL_EPI_WARPS * 2 * VL_SLAB +
-                           VL_BARRIERS;
+constexpr int VL_A_BYTES = VL_M * VL_K * 2;
+
+// Shared memory of a block, CG blocks to a tile: stages of its rows of A and its share
+// of B's columns, slabs of each epilogue warp, barriers.
+template <int CG>
+struct Block {
+  static constexpr int n = VL_N / CG;  // columns of B
+  static constexpr int stage = VL_A_BYTES + n * VL_K * 2;
+  static constexpr int stages = CG == 1 ? 4 : 5;
+  // epilogue warps, a quarter of them on each lane quarter, and the columns of each.
+  // 16 of 64 columns halve the time of a tile's stores against 8 of 128 (dW of 128
+  // tokens, whose products are short); beside one block's larger stages 8 fit.
+  static constexpr int warps = CG == 1 ? 8 : 16;
+  static constexpr int cols = VL_N * 4 / warps;
+  static constexpr int threads = 32 * (2 + warps);
+  static constexpr size_t smem = 1024 + (size_t)stages * stage + warps * VL_SLAB + 256;
+};
+static_assert(Block<1>::smem <= 227 * 1024 && Block<2>::smem <= 227 * 1024,
+              "stages exceed shared memory");
 constexpr int VL_WAIT_LIMIT = 1 << 23;  // polls (each may suspend the thread for a while)
-static_assert(VL_SMEM <= 227 * 1024, "stages exceed shared memory");
 
 __device__ int g_vocab_wait_errors;
 
@@ -90,11 +100,28 @@ struct VocabArgs {
 struct Tiles {
   int m_tiles, n_tiles, k_blocks, split_blocks, total;
 };
+struct Tile {
+  int m, n, split;
+};
+// Tokens run fastest, so that the blocks at work share W's rows; dW's rows (8 KB of a
+// 4096 wide head) are finished together: its columns run fastest.
+template <int EPI>
+__device__ __forceinline__ Tile tile_at(const Tiles &t, int i) {
+  Tile r;
+  if (EPI == EPI_OUT) {
+    r.n = i % t.n_tiles, i /= t.n_tiles;
+    r.m = i % t.m_tiles, r.split = i / t.m_tiles;
+  } else {
+    r.m = i % t.m_tiles, i /= t.m_tiles;
+    r.n = i % t.n_tiles, r.split = i / t.n_tiles;
+  }
+  return r;
+}
 template <int CG>
 __host__ __device__ inline Tiles tiles_of(const VocabArgs &a, int M, int K) {
   Tiles t;
   t.m_tiles = (M + CG * VL_M - 1) / (CG * VL_M);
-  t.n_tiles = (a.N + CG * VL_N - 1) / (CG * VL_N);
+  t.n_tiles = (a.N + VL_N - 1) / VL_N;
   t.k_blocks = (K + VL_K - 1) / VL_K;
   t.split_blocks = (t.k_blocks + a.splits - 1) / a.splits;
   t.total = t.m_tiles * t.n_tiles * a.splits;
@@ -187,10 +214,9 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, int x, int 
 __device__ __forceinline__ void store_commit() {
   asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
 }
-// all but the last `n` stores have read their shared memory
-template <int n>
+// this thread's stores have read their shared memory
 __device__ __forceinline__ void store_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(n) : "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
 }
 __device__ __forceinline__ void store_wait() {
   asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
@@ -334,24 +360,25 @@ __device__ __forceinline__ void put_floats(unsigned char *slab, int lane, const 
 // is blocks of 64 M (N) values x 64 K rows instead of rows of 64 K values.  CG: blocks
 // that share a tile.
 template <class T, int EPI, bool AMN, bool BMN, int CG>
-__global__ void __launch_bounds__(VL_THREADS, 1)
+__global__ void __launch_bounds__(Block<CG>::threads, 1)
     vocab_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_b,
                       const __grid_constant__ CUtensorMap map_out, const VocabArgs a) {
-  constexpr int TILE_M = CG * VL_M, TILE_N = CG * VL_N;
+  using B = Block<CG>;
+  constexpr int TILE_M = CG * VL_M, STAGES = B::stages;
   extern __shared__ unsigned char vl_raw[];
   unsigned char *base = vl_raw + ((1024 - (sptr(vl_raw) & 1023)) & 1023);
-  unsigned char *slabs = base + VL_STAGES * VL_STAGE;
-  uint64_t *full = reinterpret_cast<uint64_t *>(slabs + VL_EPI_WARPS * 2 * VL_SLAB);
-  uint64_t *empty = full + VL_STAGES, *acc_full = empty + VL_STAGES, *acc_empty = acc_full + 2;
+  unsigned char *slabs = base + STAGES * B::stage;
+  uint64_t *full = reinterpret_cast<uint64_t *>(slabs + B::warps * VL_SLAB);
+  uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
   uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(acc_empty + 2);
   volatile int *lost = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank = 0;
   if (CG > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
   if (threadIdx.x == 0) {
-    for (int s = 0; s < VL_STAGES; ++s) bar_init(full + s, 1), bar_init(empty + s, 1);
-    for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, CG * VL_EPI_WARPS);
+    for (int s = 0; s < STAGES; ++s) bar_init(full + s, 1), bar_init(empty + s, 1);
+    for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, CG * B::warps);
     *lost = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -359,12 +386,12 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
     if (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                        sptr(tmem_ptr)),
-                   "r"(2 * TILE_N));
+                   "r"(2 * VL_N));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     } else {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                        sptr(tmem_ptr)),
-                   "r"(2 * TILE_N));
+                   "r"(2 * VL_N));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
     }
   }
@@ -384,17 +411,17 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
       int it = 0;
       bool ok = true;
       for (int tile = first; tile < ts.total && ok; tile += step) {
-        const int mt = tile % ts.m_tiles, r = tile / ts.m_tiles;
-        const int nt = r % ts.n_tiles, split = r / ts.n_tiles;
+        const Tile at = tile_at<EPI>(ts, tile);
+        const int mt = at.m, nt = at.n, split = at.split;
         const int kb0 = split * ts.split_blocks, kb1 = min(kb0 + ts.split_blocks, ts.k_blocks);
-        const int m0 = mt * TILE_M + rank * VL_M, n0 = nt * TILE_N + rank * VL_N;
+        const int m0 = mt * TILE_M + rank * VL_M, n0 = nt * VL_N + rank * B::n;
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % VL_STAGES;
-          if (it >= VL_STAGES &&
-              !(ok = bar_wait(empty + s, ((it / VL_STAGES) - 1) & 1, lost)))
+          const int s = it % STAGES;
+          if (it >= STAGES &&
+              !(ok = bar_wait(empty + s, ((it / STAGES) - 1) & 1, lost)))
             break;
-          unsigned char *sa = base + s * VL_STAGE, *sb = sa + VL_A_BYTES;
-          if (rank == 0) bar_expect(full + s, CG * VL_STAGE);
+          unsigned char *sa = base + s * B::stage, *sb = sa + VL_A_BYTES;
+          if (rank == 0) bar_expect(full + s, CG * B::stage);
           const uint32_t bar = CG == 1 ? sptr(full + s) : in_block(full + s, 0);
           if (AMN) {
 #pragma unroll
@@ -405,7 +432,7 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
           }
           if (BMN) {
 #pragma unroll
-            for (int i = 0; i < VL_N / 64; ++i)
+            for (int i = 0; i < B::n / 64; ++i)
               tma_load<CG>(sb + i * 8192, &map_b, n0 + i * 64, a.k_first + kb * VL_K, bar);
           } else {
             tma_load<CG>(sb, &map_b, kb * VL_K, a.n_first + n0, bar);
@@ -413,8 +440,8 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
         }
       }
       if (!ok && rank == 0)  // let the loads in flight land before the block ends
-        for (int i = max(0, it - VL_STAGES); i < it; ++i)
-          for (int p = 0; p < VL_WAIT_LIMIT && !bar_try(full + i % VL_STAGES, (i / VL_STAGES) & 1);
+        for (int i = max(0, it - STAGES); i < it; ++i)
+          for (int p = 0; p < VL_WAIT_LIMIT && !bar_try(full + i % STAGES, (i / STAGES) & 1);
                ++p) {
           }
     }
@@ -422,24 +449,24 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
     if (lane == 0 && rank == 0 && sums) {
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)AMN << 15) |
-                                 ((uint32_t)BMN << 16) | ((uint32_t)(TILE_N >> 3) << 17) |
+                                 ((uint32_t)BMN << 16) | ((uint32_t)(VL_N >> 3) << 17) |
                                  ((uint32_t)(TILE_M >> 4) << 24);
       int it = 0, n = 0;
       bool ok = true;
       for (int tile = first; tile < ts.total && ok; tile += step, ++n) {
-        const int split = tile / (ts.m_tiles * ts.n_tiles);
+        const int split = tile_at<EPI>(ts, tile).split;
         const int kb0 = split * ts.split_blocks, kb1 = min(kb0 + ts.split_blocks, ts.k_blocks);
         const int buf = n & 1;
         if (n >= 2 && !(ok = bar_wait(acc_empty + buf, ((n >> 1) - 1) & 1, lost))) break;
         fence_after();
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % VL_STAGES;
-          if (!(ok = bar_wait(full + s, (it / VL_STAGES) & 1, lost))) break;
+          const int s = it % STAGES;
+          if (!(ok = bar_wait(full + s, (it / STAGES) & 1, lost))) break;
           fence_after();
-          const uint32_t sa = sptr(base + s * VL_STAGE), sb = sa + VL_A_BYTES;
+          const uint32_t sa = sptr(base + s * B::stage), sb = sa + VL_A_BYTES;
 #pragma unroll
           for (int k = 0; k < VL_K / 16; ++k)
-            mma_f16<CG>(tmem + buf * TILE_N, swizzled_desc(sa + k * (AMN ? 2048 : 32), 8192),
+            mma_f16<CG>(tmem + buf * VL_N, swizzled_desc(sa + k * (AMN ? 2048 : 32), 8192),
                         swizzled_desc(sb + k * (BMN ? 2048 : 32), 8192), idesc,
                         kb > kb0 || k > 0);
           mma_commit<CG>(empty + s);
@@ -448,19 +475,19 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
       }
     }
   } else {
-    // warps of lane quarter (warp & 3); two of them share a quarter's columns
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane;
-    constexpr int COLS = TILE_N / 2;
-    unsigned char *slab = slabs + (warp - 2) * 2 * VL_SLAB;
-    int used = 0, n = 0;
+    // warps of lane quarter (warp & 3); those of a quarter share its columns
+    const int quarter = warp & 3, part = (warp - 2) >> 2, row = quarter * 32 + lane;
+    constexpr int COLS = B::cols;
+    unsigned char *slab = slabs + (warp - 2) * VL_SLAB;
+    int n = 0;
     float scale = 1.0f;
     if constexpr (std::is_same<T, __half>::value && EPI != EPI_STATS)
       scale = dz_scale(a.tok.grad_max);
     if (EPI != EPI_DZ) scale = 1.0f / scale;
     float run_max = -INFINITY, run_sum = 0.0f;  // stats of one row over a block's tiles
     for (int tile = first; tile < ts.total; tile += step, ++n) {
-      const int mt = tile % ts.m_tiles, r = tile / ts.m_tiles;
-      const int nt = r % ts.n_tiles, split = r / ts.n_tiles;
+      const Tile where = tile_at<EPI>(ts, tile);
+      const int mt = where.m, nt = where.n, split = where.split;
       const int buf = n & 1;
       if (sums) {
         const bool ok = bar_wait(acc_full + buf, (n >> 1) & 1, lost);
@@ -468,14 +495,14 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
         fence_after();
       }
       const uint32_t acc =
-          tmem + buf * TILE_N + half * COLS + ((uint32_t)(quarter * 32) << 16);
-      const int m0 = mt * TILE_M + rank * VL_M, n0 = nt * TILE_N + half * COLS;
+          tmem + buf * VL_N + part * COLS + ((uint32_t)(quarter * 32) << 16);
+      const int m0 = mt * TILE_M + rank * VL_M, n0 = nt * VL_N + part * COLS;
       const int t = m0 + row, cols = a.N - n0;  // columns of the product from n0 on
-      // the next free slab, read out by its earlier store
+      // the slab, once its earlier store has read it
       auto next_slab = [&]() {
-        if (lane == 0) store_wait_read<1>();
+        if (lane == 0) store_wait_read();
         __syncwarp();
-        return slab + (used++ & 1) * VL_SLAB;
+        return slab;
       };
       auto filled = [&]() {
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -545,7 +572,8 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
             mx = run_max, sum = run_sum;
           }
           if (live && (!one || tile + step >= ts.total))
-            a.part[(long long)((one ? first : nt) * 2 + half) * a.M + t] = make_float2(mx, sum);
+            a.part[(long long)((one ? first : nt) * (B::warps / 4) + part) * a.M + t] =
+                make_float2(mx, sum);
         }
       } else if constexpr (EPI == EPI_PARTIAL) {
         for (int c = 0; c < COLS && c < cols; c += 32) {
@@ -598,10 +626,10 @@ __global__ void __launch_bounds__(VL_THREADS, 1)
   if (warp == 1) {
     if (CG == 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
-                   "r"(2 * TILE_N));
+                   "r"(2 * VL_N));
     else
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem),
-                   "r"(2 * TILE_N));
+                   "r"(2 * VL_N));
   }
 }
 
@@ -789,15 +817,15 @@ int launch_tiles(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap
                  const VocabArgs &a, int dev, int sms, cudaStream_t s) {
   auto k = vocab_gemm_kernel<T, EPI, AMN, BMN, CG>;
   static std::atomic<uint64_t> allowed{0};
-  if (int rc = allow_shared(k, (int)VL_SMEM, dev, allowed)) return rc;
+  if (int rc = allow_shared(k, (int)Block<CG>::smem, dev, allowed)) return rc;
   const int64_t m_tiles = (a.M + CG * VL_M - 1) / (CG * VL_M);
-  const int64_t n_tiles = (a.N + CG * VL_N - 1) / (CG * VL_N);
+  const int64_t n_tiles = (a.N + VL_N - 1) / VL_N;
   B2F_CHECK_ARG(m_tiles * n_tiles * a.splits < (1ll << 31), "b2f_vocab_loss: too many tiles");
   const int tiles = (int)(m_tiles * n_tiles * a.splits);
   cudaLaunchConfig_t c{};
   c.gridDim = dim3(CG * std::min(tiles, sms / CG));
-  c.blockDim = dim3(VL_THREADS);
-  c.dynamicSmemBytes = VL_SMEM;
+  c.blockDim = dim3(Block<CG>::threads);
+  c.dynamicSmemBytes = Block<CG>::smem;
   c.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -863,9 +891,10 @@ int gather_counted(const void *h, const Shape &z, const long long *labels, long 
 // over the ignored ones costs more than two more launches.
 bool forward_gathers(int64_t T) { return T >= 1024; }
 int64_t forward_slots(int64_t T, int64_t V, int sms) {
-  const int64_t group = blocks_per_tile(T), tiles = (V + group * VL_N - 1) / (group * VL_N);
+  const int64_t group = blocks_per_tile(T), tiles = (V + VL_N - 1) / VL_N;
+  const int per = group == 1 ? Block<1>::warps / 4 : Block<2>::warps / 4;
   // entries of blocks where one tile holds all tokens, else of tiles
-  return 2 * (T <= group * VL_M ? std::min<int64_t>(tiles, sms / group) : tiles);
+  return per * (T <= group * VL_M ? std::min<int64_t>(tiles, sms / group) : tiles);
 }
 
 // How the gradient is cut: words of a piece, splits of dh's sum over a piece.
@@ -878,7 +907,7 @@ constexpr size_t kDzBytes = 256ull << 20;
 
 Plan grad_plan(int64_t T, int64_t V, int64_t D, bool need_h, int sms) {
   Plan p{};
-  constexpr int unit = 2 * VL_N;
+  constexpr int unit = VL_N;
   int64_t words = (int64_t)(kDzBytes / 2 / (size_t)T) / unit * unit;
   words = std::max<int64_t>(words, unit);
   p.pieces = (int)((V + words - 1) / words);
@@ -889,7 +918,7 @@ Plan grad_plan(int64_t T, int64_t V, int64_t D, bool need_h, int sms) {
   // tile's store; at most 256 MB of partial sums beyond the first
   const int64_t group = blocks_per_tile(T), slots = sms / group;
   const int64_t tiles = ((T + group * VL_M - 1) / (group * VL_M)) *
-                        ((D + group * VL_N - 1) / (group * VL_N));
+                        ((D + VL_N - 1) / VL_N);
   const int64_t kb = (std::min<int64_t>(p.piece, V) + VL_K - 1) / VL_K;
   int64_t best = 0;
   p.splits = 1;
@@ -948,7 +977,7 @@ int forward(const void *h, const void *w, const Shape &z, const long long *label
   }
   CUtensorMap ma, mb;
   if (int rc = encode_map<T>(&ma, h, z.T, z.D, ldh, VL_M)) return rc;
-  if (int rc = encode_map<T>(&mb, w, z.V, z.D, z.ldw, VL_N)) return rc;
+  if (int rc = encode_map<T>(&mb, w, z.V, z.D, z.ldw, VL_N / group)) return rc;
   if (int rc = launch_gemm<T, EPI_STATS, false, false>(ma, mb, ma, a, group, dev, sms, s))
     return rc;
   vocab_join_kernel<<<(z.T + 7) / 8, dim3(8, 64), 0, s>>>(a.part, a.label_logit, labels, ignore,
@@ -968,7 +997,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
   const int group = blocks_per_tile(z.T);
   CUtensorMap h_k, h_n, w_k, w_n, dz_k, dz_m, dz_out, sums, dw_out;
   if (int rc = encode_map<T>(&h_k, hc, z.T, z.D, z.D, VL_M)) return rc;
-  if (int rc = encode_map<T>(&w_k, w, z.V, z.D, z.ldw, VL_N)) return rc;
+  if (int rc = encode_map<T>(&w_k, w, z.V, z.D, z.ldw, VL_N / group)) return rc;
   if (int rc = encode_map<T>(&h_n, hc, z.T, z.D, z.D, VL_K)) return rc;
   if (int rc = encode_map<T>(&w_n, w, z.V, z.D, z.ldw, VL_K)) return rc;
   if (dh)
@@ -1000,7 +1029,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
       b.M = words, b.N = z.D, b.K = z.T, b.splits = 1;
       b.m_first = v0;
       b.tok = tok, b.tokens_in_k = 1;
-      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, dw_out, b, group, dev, sms, s))
+      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, dw_out, b, 2, dev, sms, s))
         return rc;
     }
   }
