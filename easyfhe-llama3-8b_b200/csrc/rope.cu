@@ -8,15 +8,21 @@
 // the negative angle.
 //
 // Bytes bound: every element is read and written once, 3 operations each.  A
-// block takes TB tokens: its threads first compute the r/2 (c, s) of each
-// token into shared memory (once per token, for all of its heads), then each
-// thread keeps the (c, s) of its 16 bytes of pairs in registers and runs over
-// the heads.  The angle of a far position needs more than binary32: p f is
+// block takes up to ROPE_TOKENS tokens of a sequence (one where there are few): its
+// threads first compute the r/2 (c, s) of each token into shared memory (once per
+// token, for all of its heads), then each thread keeps the (c, s) of its 16 bytes
+// of pairs in registers and runs over the heads.  What paid beside that: sequences
+// on the grid's second dimension, because a 64-bit division by their length per
+// token and thread took more instructions than the rotation (32768 tokens of 40
+// heads of 128 in bf16: 159 us with it, 109 without, 94 % of copy bandwidth), and
+// registers for five blocks of 256 threads on an SM (four with two heads in flight
+// per thread: 129 us).
+// The angle of a far position needs more than binary32: p f is
 // formed in binary64 and reduced there to a fraction of a turn in [-1/2,
 // 1/2], whose sine and cosine are then taken in binary32 (the reduction's
 // error is 2^-52 of the turns, the rounding of the fraction 2^-25 of a turn);
 // binary64 inputs take binary64 sines of p f.
-#include "b2f_internal.h"
+#include "plain.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,7 +30,7 @@
 namespace b2f {
 namespace {
 
-constexpr int ROPE_TOKENS = 4;     // tokens of a block
+constexpr int ROPE_TOKENS = 4;     // tokens of a block, at most
 constexpr int ROPE_THREADS = 256;  // at most
 
 struct RopePart {
@@ -35,7 +41,8 @@ struct RopePart {
 struct RopeArgs {
   RopePart part[2];
   int heads0, heads;  // heads of part 0, of both
-  long long tokens, seq;
+  int block_tokens;
+  long long batch, seq;
   int dim, rotary, interleaved;
   const void *pos;
   int pos64;
@@ -94,6 +101,16 @@ __device__ __forceinline__ void turn_of(double p, double f, double factor, int s
   o = make_double2(c * factor, (double)sign * s * factor);
 }
 
+// two roundings at once
+__device__ __forceinline__ void put2(__nv_bfloat16 *o, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162 *>(o) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void put2(__half *o, float a, float b) {
+  *reinterpret_cast<__half2 *>(o) = __floats2half2_rn(a, b);
+}
+__device__ __forceinline__ void put2(float *o, float a, float b) { o[0] = a, o[1] = b; }
+__device__ __forceinline__ void put2(double *o, double a, double b) { o[0] = a, o[1] = b; }
+
 template <class T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
@@ -102,80 +119,96 @@ struct alignas(sizeof(T) * VEC) Pack {
 // block (x: 16-byte units of a head, y: heads), grid: ROPE_TOKENS tokens each.
 // VEC elements per access; units [0, rot_units) rotate, the rest copy.
 template <class T, int VEC>
-__global__ void __launch_bounds__(ROPE_THREADS)
+__global__ void __launch_bounds__(ROPE_THREADS, 5)
     rope_kernel(const RopeArgs a, int rot_units, int units) {
   using W = typename Wide<T>::V;
   using W2 = typename Wide<T>::V2;
   extern __shared__ __align__(16) unsigned char rope_smem[];
-  W2 *cs = reinterpret_cast<W2 *>(rope_smem);
   const int half = a.rotary / 2;
-  const long long t0 = (long long)blockIdx.x * ROPE_TOKENS;
-  const int nt = (int)min((long long)ROPE_TOKENS, a.tokens - t0);
-  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
-  for (int i = tid; i < nt * half; i += blockDim.x * blockDim.y) {
-    const int t = i / half, j = i - t * half;
-    const long long tok = t0 + t, b = tok / a.seq, s = tok - b * a.seq;
-    const long long at = b * a.pos_b + s * a.pos_s;
-    const double p = a.pos64 ? (double)static_cast<const long long *>(a.pos)[at]
-                             : (double)static_cast<const int *>(a.pos)[at];
-    turn_of(p, a.freqs[j], (W)a.factor, a.sign, cs[i]);
-  }
-  __syncthreads();
+  // (c, s) of the block's tokens, cosines and sines apart
+  W *cosines = reinterpret_cast<W *>(rope_smem), *sines = cosines + a.block_tokens * half;
   using P = Pack<T, VEC>;
-  for (int t = 0; t < nt; ++t) {
-    const long long tok = t0 + t, b = tok / a.seq, s = tok - b * a.seq;
-    for (int u = threadIdx.x; u < units; u += blockDim.x) {
-      const bool rot = u < rot_units;
-      // pairs of this unit: half layout VEC of them, interleaved VEC / 2 (1 for VEC 1)
-      constexpr int NP = VEC;
-      W2 c[NP];
-      int e0, e1 = 0;  // element offsets of the unit's accesses
-      const int pairs = a.interleaved ? (VEC > 1 ? VEC / 2 : 1) : VEC;
-      if (rot) {
-        e0 = a.interleaved ? u * pairs * 2 : u * VEC;
-        e1 = a.interleaved ? e0 + 1 : e0 + half;
-#pragma unroll
-        for (int k = 0; k < NP; ++k)
-          if (k < pairs) c[k] = cs[t * half + u * pairs + k];
-      } else {
-        e0 = a.rotary + (u - rot_units) * VEC;
-      }
-      for (int h = threadIdx.y; h < a.heads; h += blockDim.y) {
-        const bool second = h >= a.heads0;
-        const RopePart &pt = second ? a.part[1] : a.part[0];
-        const int hh = second ? h - a.heads0 : h;
-        const T *in = static_cast<const T *>(pt.in) + b * pt.ib + s * pt.is + hh * pt.ih;
-        T *out = static_cast<T *>(pt.out) + b * pt.ob + s * pt.os + hh * pt.oh;
-        const P x0 = *reinterpret_cast<const P *>(in + e0);
-        P y0 = x0;
+  // pairs of a unit: half layout VEC of them, interleaved VEC / 2 (1 for VEC 1)
+  const int pairs = a.interleaved && VEC > 1 ? VEC / 2 : VEC;
+  const bool two = !(VEC > 1 && a.interleaved);  // a rotated unit is two accesses
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const long long s0 = (long long)blockIdx.x * a.block_tokens;
+  const int nt = (int)min((long long)a.block_tokens, a.seq - s0);
+  for (long long b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    for (int i = tid; i < nt * half; i += blockDim.x * blockDim.y) {
+      const int t = i / half, j = i - t * half;
+      const long long at = b * a.pos_b + (s0 + t) * a.pos_s;
+      const double p = a.pos64 ? (double)static_cast<const long long *>(a.pos)[at]
+                               : (double)static_cast<const int *>(a.pos)[at];
+      W2 cs;
+      turn_of(p, a.freqs[j], (W)a.factor, a.sign, cs);
+      cosines[i] = cs.x;
+      sines[i] = cs.y;
+    }
+    __syncthreads();
+    const T *in0 = static_cast<const T *>(a.part[0].in) + b * a.part[0].ib + s0 * a.part[0].is;
+    const T *in1 = static_cast<const T *>(a.part[1].in) + b * a.part[1].ib + s0 * a.part[1].is;
+    T *out0 = static_cast<T *>(a.part[0].out) + b * a.part[0].ob + s0 * a.part[0].os;
+    T *out1 = static_cast<T *>(a.part[1].out) + b * a.part[1].ob + s0 * a.part[1].os;
+    for (int t = 0; t < nt; ++t) {
+      for (int u = threadIdx.x; u < units; u += blockDim.x) {
+        const bool rot = u < rot_units;
+        W c[VEC], n[VEC];
+        int e0, e1 = 0;  // element offsets of the unit's accesses
         if (rot) {
-          if (VEC > 1 && a.interleaved) {
+          e0 = a.interleaved ? u * pairs * 2 : u * VEC;
+          e1 = a.interleaved ? e0 + 1 : e0 + half;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            if (k < pairs) {
+              c[k] = cosines[t * half + u * pairs + k];
+              n[k] = sines[t * half + u * pairs + k];
+            }
+        } else {
+          e0 = a.rotary + (u - rot_units) * VEC;
+        }
+        for (int h = threadIdx.y; h < a.heads; h += blockDim.y) {
+          const bool first = h < a.heads0;
+          const T *in = first ? in0 + h * a.part[0].ih : in1 + (h - a.heads0) * a.part[1].ih;
+          T *out = first ? out0 + h * a.part[0].oh : out1 + (h - a.heads0) * a.part[1].oh;
+          const P x0 = *reinterpret_cast<const P *>(in + e0);
+          P y0 = x0;
+          if (rot && two) {
+            const P x1 = *reinterpret_cast<const P *>(in + e1);
+            P y1;
+            if constexpr (VEC == 1) {
+              const W lo = to_wide(x0.v[0]), hi = to_wide(x1.v[0]);
+              y0.v[0] = from_wide<T>(lo * c[0] - hi * n[0]);
+              y1.v[0] = from_wide<T>(hi * c[0] + lo * n[0]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < VEC; k += 2) {
+                const W lo = to_wide(x0.v[k]), hi = to_wide(x1.v[k]);
+                const W lo1 = to_wide(x0.v[k + 1]), hi1 = to_wide(x1.v[k + 1]);
+                put2(y0.v + k, lo * c[k] - hi * n[k], lo1 * c[k + 1] - hi1 * n[k + 1]);
+                put2(y1.v + k, hi * c[k] + lo * n[k], hi1 * c[k + 1] + lo1 * n[k + 1]);
+              }
+            }
+            *reinterpret_cast<P *>(out + e1) = y1;
+          } else if (rot) {
 #pragma unroll
             for (int k = 0; k < VEC / 2; ++k) {
               const W lo = to_wide(x0.v[2 * k]), hi = to_wide(x0.v[2 * k + 1]);
-              y0.v[2 * k] = from_wide<T>(lo * c[k].x - hi * c[k].y);
-              y0.v[2 * k + 1] = from_wide<T>(hi * c[k].x + lo * c[k].y);
+              put2(y0.v + 2 * k, lo * c[k] - hi * n[k], hi * c[k] + lo * n[k]);
             }
-          } else {
-            const P x1 = *reinterpret_cast<const P *>(in + e1);
-            P y1;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const W lo = to_wide(x0.v[k]), hi = to_wide(x1.v[k]);
-              y0.v[k] = from_wide<T>(lo * c[k].x - hi * c[k].y);
-              y1.v[k] = from_wide<T>(hi * c[k].x + lo * c[k].y);
-            }
-            *reinterpret_cast<P *>(out + e1) = y1;
           }
+          *reinterpret_cast<P *>(out + e0) = y0;
         }
-        *reinterpret_cast<P *>(out + e0) = y0;
       }
+      in0 += a.part[0].is, in1 += a.part[1].is;
+      out0 += a.part[0].os, out1 += a.part[1].os;
     }
+    __syncthreads();  // before the next sequence's angles
   }
 }
 
 template <class T>
-int launch_rope(const RopeArgs &a, int parts, cudaStream_t s) {
+int launch_rope(RopeArgs a, int parts, int sms, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const int half = a.rotary / 2;
   bool vec = a.dim % V == 0 && a.rotary % V == 0 && (a.interleaved || half % V == 0);
@@ -194,8 +227,11 @@ int launch_rope(const RopeArgs &a, int parts, cudaStream_t s) {
   const int passes = (a.heads * bx + ROPE_THREADS - 1) / ROPE_THREADS;
   const int by = std::min((a.heads + passes - 1) / passes, ROPE_THREADS / bx);
   const dim3 block(bx, by);
-  const unsigned grid = (unsigned)((a.tokens + ROPE_TOKENS - 1) / ROPE_TOKENS);
-  const size_t smem = (size_t)ROPE_TOKENS * half * 2 * sizeof(typename Wide<T>::V);
+  // few tokens: one to a block; more share a block's pipeline
+  a.block_tokens = (int)std::max<long long>(1, std::min<long long>(ROPE_TOKENS, a.batch * a.seq / (8 * sms)));
+  const dim3 grid((unsigned)((a.seq + a.block_tokens - 1) / a.block_tokens),
+                  (unsigned)std::min<long long>(a.batch, 65535));
+  const size_t smem = (size_t)a.block_tokens * half * 2 * sizeof(typename Wide<T>::V);
   if (vec)
     rope_kernel<T, V><<<grid, block, smem, s>>>(a, rot_units, units);
   else
@@ -233,8 +269,8 @@ extern "C" int b2f_rope(const b2f_rope_heads *parts, int num_parts, int dtype, i
   }
   B2F_CHECK_ARG(dtype >= B2F_F64 && dtype <= B2F_BF16, "b2f_rope: dtype %d", dtype);
   if (batch == 0 || seq == 0) return B2F_OK;
-  B2F_CHECK_ARG(seq <= (1ll << 32) / batch, "b2f_rope: %lld x %lld tokens", (long long)batch,
-                (long long)seq);
+  B2F_CHECK_ARG(seq < (1ll << 31) && batch < (1ll << 31), "b2f_rope: %lld x %lld tokens",
+                (long long)batch, (long long)seq);
   B2F_CHECK_ARG(positions && freqs, "b2f_rope: null positions or frequencies");
   const uintptr_t size = dtype == B2F_F64 ? 8 : dtype == B2F_F32 ? 4 : 2;
   for (int i = 0; i < num_parts; ++i)
@@ -243,7 +279,7 @@ extern "C" int b2f_rope(const b2f_rope_heads *parts, int num_parts, int dtype, i
                   "b2f_rope: null or misaligned heads");
   a.heads0 = parts[0].heads;
   a.heads = (int)heads;
-  a.tokens = batch * seq;
+  a.batch = batch;
   a.seq = seq;
   a.dim = dim;
   a.rotary = rotary;
@@ -255,15 +291,17 @@ extern "C" int b2f_rope(const b2f_rope_heads *parts, int num_parts, int dtype, i
   a.freqs = freqs;
   a.factor = factor;
   a.sign = gradient ? -1 : 1;
+  int dev = 0, sms = 0;
+  if (int rc = current_device(&dev, &sms)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case B2F_F64:
-      return launch_rope<double>(a, num_parts, s);
+      return launch_rope<double>(a, num_parts, sms, s);
     case B2F_F32:
-      return launch_rope<float>(a, num_parts, s);
+      return launch_rope<float>(a, num_parts, sms, s);
     case B2F_F16:
-      return launch_rope<__half>(a, num_parts, s);
+      return launch_rope<__half>(a, num_parts, sms, s);
     default:
-      return launch_rope<__nv_bfloat16>(a, num_parts, s);
+      return launch_rope<__nv_bfloat16>(a, num_parts, sms, s);
   }
 }

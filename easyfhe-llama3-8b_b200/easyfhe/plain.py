@@ -171,22 +171,18 @@ def _rope_refuse(what, q, k, positions, plan):
                      f"{tuple(q.shape[:-2])}")
 
 
-def _rope_part(plan, t, outer):
-    """(packed b2f_rope_heads, output, input kept alive) of one tensor, None to refuse."""
+def _rope_part(t, shape):
+    """(packed b2f_rope_heads, output, input kept alive) of one tensor."""
 
-    shape = t.shape
-    if shape[-1] != plan.head_dim or shape[:-2] != outer or not 1 <= shape[-2] <= 4096:
-        return None
     st = t.stride()
     if st[-1] != 1:
         t = t.contiguous()
         st = t.stride()
+    out = torch.empty_like(t, memory_format=torch.contiguous_format)
     heads, dim = shape[-2], shape[-1]
-    out = t.new_empty(shape)
     row = heads * dim
-    batch = st[0] if len(shape) == 4 else 0
-    return _HEADS.pack(t.data_ptr(), out.data_ptr(), batch, st[-3], st[-2],
-                       row * shape[-3], row, dim, heads), out, t
+    return _HEADS.pack(t.data_ptr(), out.data_ptr(), st[0] if len(shape) == 4 else 0, st[-3],
+                       st[-2], row * shape[-3], row, dim, heads), out, t
 
 
 def _rope(what, q, k, positions, plan, gradient):
@@ -198,17 +194,19 @@ def _rope(what, q, k, positions, plan, gradient):
     if _current_device() != plan.index:
         with torch.cuda.device(plan.index):
             return _rope(what, q, k, positions, plan, gradient)
-    outer = q.shape[:-2]
+    shape = tuple(q.shape)
+    outer = shape[:-2]
     batch, seq = outer if len(outer) == 2 else (1, outer[0])
     pos = positions.stride()
     wide = positions.dtype is torch.int64
-    if not (wide or positions.dtype is torch.int32) or \
-            tuple(positions.shape) not in ((seq,), (batch, seq)):
+    kshape = shape if k is None else tuple(k.shape)
+    if not (wide or positions.dtype is torch.int32) \
+            or tuple(positions.shape) not in ((seq,), (batch, seq)) \
+            or shape[-1] != plan.head_dim or kshape[-1] != plan.head_dim \
+            or kshape[:-2] != outer or not 1 <= shape[-2] <= 4096 or not 1 <= kshape[-2] <= 4096:
         _rope_refuse(what, q, k, positions, plan)
-    a = _rope_part(plan, q, outer)
-    b = None if k is None else _rope_part(plan, k, outer)
-    if a is None or (b is None and k is not None):
-        _rope_refuse(what, q, k, positions, plan)
+    a = _rope_part(q, shape)
+    b = None if k is None else _rope_part(k, kshape)
     if batch and seq:
         rc = lib.b2f_rope(a[0] if b is None else a[0] + b[0], 1 if b is None else 2,
                           _DTYPES[q.dtype], batch, seq, plan.head_dim, plan.rotary_dim,
@@ -472,8 +470,9 @@ def vocab_loss_grad(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
                                    need_weight=need_weight)
     h, w, lab = _rows16(hidden, d), _rows16(weight, d), labels.contiguous()
     lse, g = lse.contiguous(), grad_loss.contiguous()
-    dh = h.new_empty((t, d)) if need_hidden else None
-    dw = w.new_empty((v, d)) if need_weight else None
+    like = torch.contiguous_format
+    dh = torch.empty_like(h, memory_format=like) if need_hidden else None
+    dw = torch.empty_like(w, memory_format=like) if need_weight else None
     ws = h.new_empty((max(lib.b2f_vocab_loss_grad_workspace(t, v, d, bool(need_hidden)), 16),),
                      dtype=torch.uint8)
     rc = lib.b2f_vocab_loss_grad(h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
