@@ -31,4 +31,46 @@ int allow_shared(K kernel, int bytes, int dev, std::atomic<uint64_t> &done) {
   return B2F_OK;
 }
 
+// Launches a kernel of a chain.  `chained`: it may start while the kernel before it
+// in the stream still runs (programmatic dependent launch); every thread block of such
+// a kernel, and of the one it follows, passes wait_for_previous before it touches what
+// that one writes, so a kernel has ended only when all before it have.
+template <class... P, class... A>
+int launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, int cluster,
+                   bool chained, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = shared;
+  c.stream = s;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (chained) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  c.attrs = at;
+  c.numAttrs = n;
+  B2F_CUDA(cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...));
+  note_launch();
+  return B2F_OK;
+}
+#ifdef __CUDACC__
+// the kernel after this one in the stream may start
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+}
+// all that the kernel before this one wrote is there
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+#endif
+
 }  // namespace b2f

@@ -14,11 +14,11 @@
 // of pairs in registers and runs over the heads.  What paid beside that: sequences
 // on the grid's second dimension, because a 64-bit division by their length per
 // token and thread took more instructions than the rotation (32768 tokens of 40
-// heads of 128 in bf16: 159 us with it, 109 without, 94 % of copy bandwidth), and
-// registers for five blocks of 256 threads on an SM (four with two heads in flight
-// per thread: 129 us).
-// The angle of a far position needs more than binary32: p f is
-// formed in binary64 and reduced there to a fraction of a turn in [-1/2,
+// heads of 128 in bf16: 159 us with it, 109 without, 94 % of copy bandwidth), both
+// loads of a head before anything else of it (131 us with the second one after the
+// output's address), and registers for five blocks of 256 threads on an SM (four
+// with two heads in flight per thread: 129 us).
+// The angle of a far position needs more than binary32: p f is formed in binary64 and reduced there to a fraction of a turn in [-1/2,
 // 1/2], whose sine and cosine are then taken in binary32 (the reduction's
 // error is 2^-52 of the turns, the rounding of the fraction 2^-25 of a turn);
 // binary64 inputs take binary64 sines of p f.
@@ -167,14 +167,16 @@ __global__ void __launch_bounds__(ROPE_THREADS, 5)
         } else {
           e0 = a.rotary + (u - rot_units) * VEC;
         }
+#pragma unroll 1
         for (int h = threadIdx.y; h < a.heads; h += blockDim.y) {
           const bool first = h < a.heads0;
           const T *in = first ? in0 + h * a.part[0].ih : in1 + (h - a.heads0) * a.part[1].ih;
+          P x0, x1;
+          x0 = *reinterpret_cast<const P *>(in + e0);
+          if (rot && two) x1 = *reinterpret_cast<const P *>(in + e1);
           T *out = first ? out0 + h * a.part[0].oh : out1 + (h - a.heads0) * a.part[1].oh;
-          const P x0 = *reinterpret_cast<const P *>(in + e0);
           P y0 = x0;
           if (rot && two) {
-            const P x1 = *reinterpret_cast<const P *>(in + e1);
             P y1;
             if constexpr (VEC == 1) {
               const W lo = to_wide(x0.v[0]), hi = to_wide(x1.v[0]);

@@ -302,7 +302,7 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 // power of two S with S max|g| in [2^13, 2^14] (1 for a zero, infinite or NaN
 // maximum): dz is formed times S for fp16
 __device__ __forceinline__ float dz_scale(const uint32_t *grad_max) {
-  const int e = (int)(__ldg(grad_max) >> 23);  // sign bit clear
+  const int e = (int)(*grad_max >> 23);  // sign bit clear
   if (e == 0 || e == 255) return 1.0f;
   const int k = min(max(127 + 13 - (e - 127), 1), 254);
   return __uint_as_float((uint32_t)k << 23);
@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
   uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(acc_empty + 2);
   volatile int *lost = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  let_next_start();
   uint32_t rank = 0;
   if (CG > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
   if (threadIdx.x == 0) {
@@ -400,6 +401,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
   if (CG > 1) cluster_meet();
   fence_after();
   const uint32_t tmem = *tmem_ptr;
+  wait_for_previous();
   int M = a.M, K = a.K;
   if (a.tok.count) (a.tokens_in_k ? K : M) = *a.tok.count;
   const Tiles ts = tiles_of<CG>(a, M, K);
@@ -641,6 +643,8 @@ __global__ void __launch_bounds__(512)
                       const int *__restrict__ place, int T, int slots, float *__restrict__ loss,
                       float *__restrict__ lse) {
   __shared__ float2 sm[64][9];
+  let_next_start();
+  wait_for_previous();
   const int t = blockIdx.x * 8 + threadIdx.x;
   const bool live = t < T && labels[t] != ignore;
   const int at = live ? (place ? place[t] : t) : 0;
@@ -674,6 +678,8 @@ __global__ void __launch_bounds__(1024)
                        int *__restrict__ count, uint32_t *__restrict__ grad_max) {
   __shared__ int sums[32];
   __shared__ uint32_t tops[32];
+  let_next_start();
+  wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int before = 0;
   uint32_t top = 0;
@@ -716,6 +722,8 @@ __global__ void __launch_bounds__(128)
                         const float *__restrict__ grad, T *__restrict__ out,
                         long long *__restrict__ out_labels, float *__restrict__ out_lse,
                         float *__restrict__ out_grad) {
+  let_next_start();
+  wait_for_previous();
   const int t = blockIdx.x, p = place[t];
   if (p >= 0) {
     const uint4 *in = reinterpret_cast<const uint4 *>(h + t * ldh);
@@ -733,24 +741,31 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// Sum of the splits' dh, in order, rounded once; zero rows for ignored tokens.
+// Sum of the splits' dh, rounded once; zero rows for ignored tokens.  Four threads share
+// the splits of four columns, and their sums are added in order.
 template <class T>
 __global__ void __launch_bounds__(256)
     vocab_sum_kernel(const float4 *__restrict__ partial, int splits, int tokens, int d4,
                      const int *__restrict__ place, const uint32_t *__restrict__ grad_max,
                      uint2 *__restrict__ out) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)tokens * d4) return;
-  const int t = (int)(i / d4), c = (int)(i - (long long)t * d4), p = place[t];
+  __shared__ float4 sm[3][64];
+  let_next_start();
+  wait_for_previous();
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const long long i = (long long)blockIdx.x * 64 + x, n = (long long)tokens * d4;
+  const int t = i < n ? (int)(i / d4) : 0, c = (int)(i - (long long)t * d4);
+  const int p = i < n ? place[t] : -1;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](const float4 &w) { v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w; };
   if (p >= 0) {
     const float4 *from = partial + (long long)p * d4 + c;
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) {
-      const float4 w = from[(long long)s * tokens * d4];
-      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-    }
+#pragma unroll 4
+    for (int s = y; s < splits; s += 4) add(from[(long long)s * n]);
   }
+  if (y) sm[y - 1][x] = v;
+  __syncthreads();
+  if (y || i >= n) return;
+  for (int k = 0; k < 3; ++k) add(sm[k][x]);
   float scale = 1.0f;
   if constexpr (std::is_same<T, __half>::value) scale = 1.0f / dz_scale(grad_max);
   out[i] = make_uint2(pack2<T>(v.x * scale, v.y * scale), pack2<T>(v.z * scale, v.w * scale));
@@ -814,7 +829,7 @@ int blocks_per_tile(int64_t T) { return T > VL_M ? 2 : 1; }
 
 template <class T, int EPI, bool AMN, bool BMN, int CG>
 int launch_tiles(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo,
-                 const VocabArgs &a, int dev, int sms, cudaStream_t s) {
+                 const VocabArgs &a, bool chained, int dev, int sms, cudaStream_t s) {
   auto k = vocab_gemm_kernel<T, EPI, AMN, BMN, CG>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared(k, (int)Block<CG>::smem, dev, allowed)) return rc;
@@ -822,26 +837,14 @@ int launch_tiles(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap
   const int64_t n_tiles = (a.N + VL_N - 1) / VL_N;
   B2F_CHECK_ARG(m_tiles * n_tiles * a.splits < (1ll << 31), "b2f_vocab_loss: too many tiles");
   const int tiles = (int)(m_tiles * n_tiles * a.splits);
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(CG * std::min(tiles, sms / CG));
-  c.blockDim = dim3(Block<CG>::threads);
-  c.dynamicSmemBytes = Block<CG>::smem;
-  c.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  c.attrs = at;
-  c.numAttrs = CG > 1 ? 1 : 0;
-  B2F_CUDA(cudaLaunchKernelEx(&c, k, ma, mb, mo, a));
-  B2F_LAUNCHED("vocab_gemm_kernel");
-  return B2F_OK;
+  return launch_chained(k, dim3(CG * std::min(tiles, sms / CG)), dim3(Block<CG>::threads),
+                        Block<CG>::smem, CG, chained, s, ma, mb, mo, a);
 }
 template <class T, int EPI, bool AMN, bool BMN>
 int launch_gemm(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo,
-                const VocabArgs &a, int group, int dev, int sms, cudaStream_t s) {
-  return group == 2 ? launch_tiles<T, EPI, AMN, BMN, 2>(ma, mb, mo, a, dev, sms, s)
-                    : launch_tiles<T, EPI, AMN, BMN, 1>(ma, mb, mo, a, dev, sms, s);
+                const VocabArgs &a, int group, bool chained, int dev, int sms, cudaStream_t s) {
+  return group == 2 ? launch_tiles<T, EPI, AMN, BMN, 2>(ma, mb, mo, a, chained, dev, sms, s)
+                    : launch_tiles<T, EPI, AMN, BMN, 1>(ma, mb, mo, a, chained, dev, sms, s);
 }
 
 struct Shape {
@@ -877,12 +880,14 @@ int gather_counted(const void *h, const Shape &z, const long long *labels, long 
   auto *gmax = reinterpret_cast<uint32_t *>(ws + c.gmax);
   auto *lab = reinterpret_cast<long long *>(ws + c.labels);
   float *l = reinterpret_cast<float *>(ws + c.lse), *g = reinterpret_cast<float *>(ws + c.grad);
-  vocab_count_kernel<<<1, 1024, 0, s>>>(labels, ignore, grad, z.T, place, count, gmax);
-  B2F_LAUNCHED("vocab_count_kernel");
-  vocab_gather_kernel<T><<<z.T, 128, 0, s>>>(static_cast<const T *>(h), z.ldh, z.D, z.T, place,
-                                             count, labels, lse, grad,
-                                             reinterpret_cast<T *>(ws + c.rows), lab, l, g);
-  B2F_LAUNCHED("vocab_gather_kernel");
+  // the first of its chain: it waits for all before it
+  if (int rc = launch_chained(vocab_count_kernel, dim3(1), dim3(1024), 0, 1, false, s, labels,
+                              ignore, grad, z.T, place, count, gmax))
+    return rc;
+  if (int rc = launch_chained(vocab_gather_kernel<T>, dim3(z.T), dim3(128), 0, 1, true, s,
+                              static_cast<const T *>(h), z.ldh, z.D, z.T, place, count, labels,
+                              lse, grad, reinterpret_cast<T *>(ws + c.rows), lab, l, g))
+    return rc;
   *tok = Counted{count, lab, l, g, gmax};
   return B2F_OK;
 }
@@ -978,12 +983,11 @@ int forward(const void *h, const void *w, const Shape &z, const long long *label
   CUtensorMap ma, mb;
   if (int rc = encode_map<T>(&ma, h, z.T, z.D, ldh, VL_M)) return rc;
   if (int rc = encode_map<T>(&mb, w, z.V, z.D, z.ldw, VL_N / group)) return rc;
-  if (int rc = launch_gemm<T, EPI_STATS, false, false>(ma, mb, ma, a, group, dev, sms, s))
+  if (int rc = launch_gemm<T, EPI_STATS, false, false>(ma, mb, ma, a, group, place != nullptr, dev,
+                                                     sms, s))
     return rc;
-  vocab_join_kernel<<<(z.T + 7) / 8, dim3(8, 64), 0, s>>>(a.part, a.label_logit, labels, ignore,
-                                                          z.V, place, z.T, (int)slots, loss, lse);
-  B2F_LAUNCHED("vocab_join_kernel");
-  return B2F_OK;
+  return launch_chained(vocab_join_kernel, dim3((z.T + 7) / 8), dim3(8, 64), 0, 1, true, s, a.part,
+                        a.label_logit, labels, ignore, z.V, place, z.T, (int)slots, loss, lse);
 }
 
 template <class T>
@@ -1011,7 +1015,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
     a.n_first = v0;
     a.tok = tok, a.ignore = ignore, a.vocab = z.V;
     if (int rc = encode_map<T>(&dz_out, dz, z.T, words, p.piece, 32)) return rc;
-    if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, dz_out, a, group, dev, sms, s))
+    if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, dz_out, a, group, true, dev, sms, s))
       return rc;
     if (dh) {
       if (int rc = encode_map<T>(&dz_k, dz, z.T, words, p.piece, VL_M)) return rc;
@@ -1020,7 +1024,8 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
       b.k_first = v0;
       b.tok = tok;
       b.accumulate = i > 0;
-      if (int rc = launch_gemm<T, EPI_PARTIAL, false, true>(dz_k, w_n, sums, b, group, dev, sms, s))
+      if (int rc = launch_gemm<T, EPI_PARTIAL, false, true>(dz_k, w_n, sums, b, group, true, dev, sms,
+                                                         s))
         return rc;
     }
     if (dw) {
@@ -1029,16 +1034,16 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
       b.M = words, b.N = z.D, b.K = z.T, b.splits = 1;
       b.m_first = v0;
       b.tok = tok, b.tokens_in_k = 1;
-      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, dw_out, b, 2, dev, sms, s))
+      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, dw_out, b, 2, true, dev, sms, s))
         return rc;
     }
   }
   if (dh) {
     const long long n4 = (long long)z.T * z.D / 4;
-    vocab_sum_kernel<T><<<(unsigned)((n4 + 255) / 256), 256, 0, s>>>(
-        reinterpret_cast<const float4 *>(partial), p.splits, z.T, z.D / 4,
-        reinterpret_cast<const int *>(ws + p.c.place), tok.grad_max, static_cast<uint2 *>(dh));
-    B2F_LAUNCHED("vocab_sum_kernel");
+    return launch_chained(vocab_sum_kernel<T>, dim3((unsigned)((n4 + 63) / 64)), dim3(256), 0, 1,
+                          true, s, reinterpret_cast<const float4 *>(partial), p.splits, z.T,
+                          z.D / 4, reinterpret_cast<const int *>(ws + p.c.place), tok.grad_max,
+                          static_cast<uint2 *>(dh));
   }
   return B2F_OK;
 }
