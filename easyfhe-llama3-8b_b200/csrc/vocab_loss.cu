@@ -713,18 +713,51 @@ __global__ void __launch_bounds__(1024)
 }
 
 // The counted tokens' rows, labels, lse and g, packed; up to 63 zero rows behind them
-// fill the last K block of dW.
-template <class T>
+// fill the last K block of dW.  SELF: each block counts for itself (few tokens), and
+// vocab_count_kernel's results are written here.
+template <class T, bool SELF>
 __global__ void __launch_bounds__(128)
-    vocab_gather_kernel(const T *__restrict__ h, long long ldh, int D, int tokens,
-                        const int *__restrict__ place, const int *__restrict__ count,
-                        const long long *__restrict__ labels, const float *__restrict__ lse,
+    vocab_gather_kernel(const T *__restrict__ h, long long ldh, int D, int tokens, int *place,
+                        int *count, uint32_t *grad_max, const long long *__restrict__ labels,
+                        long long ignore, const float *__restrict__ lse,
                         const float *__restrict__ grad, T *__restrict__ out,
                         long long *__restrict__ out_labels, float *__restrict__ out_lse,
                         float *__restrict__ out_grad) {
+  __shared__ int sums[4][2];
+  __shared__ uint32_t tops[4];
   let_next_start();
-  wait_for_previous();
-  const int t = blockIdx.x, p = place[t];
+  const int t = blockIdx.x;
+  int p, total;
+  if (SELF) {
+    int before = 0, all = 0;
+    uint32_t top = 0;
+    for (int i = threadIdx.x; i < tokens; i += 128) {
+      const bool in = labels[i] != ignore;
+      all += in;
+      before += in && i < t;
+      if (in && grad) top = max(top, __float_as_uint(fabsf(grad[i])));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      all += __shfl_xor_sync(~0u, all, o);
+      before += __shfl_xor_sync(~0u, before, o);
+      top = max(top, __shfl_xor_sync(~0u, top, o));
+    }
+    const int w = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) sums[w][0] = before, sums[w][1] = all, tops[w] = top;
+    __syncthreads();
+    before = sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0];
+    total = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
+    p = labels[t] != ignore ? before : -1;
+    if (threadIdx.x == 0) {
+      place[t] = p;
+      if (t == 0) *count = total, *grad_max = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
+  } else {
+    wait_for_previous();
+    p = place[t];
+    total = *count;
+  }
   if (p >= 0) {
     const uint4 *in = reinterpret_cast<const uint4 *>(h + t * ldh);
     uint4 *o = reinterpret_cast<uint4 *>(out + (long long)p * D);
@@ -734,7 +767,7 @@ __global__ void __launch_bounds__(128)
       if (lse) out_lse[p] = lse[t], out_grad[p] = grad[t];
     }
   }
-  const int zero = *count + t;
+  const int zero = total + t;
   if (t < 63 && zero < tokens) {
     uint4 *o = reinterpret_cast<uint4 *>(out + (long long)zero * D);
     for (int i = threadIdx.x; i < D / 8; i += 128) o[i] = make_uint4(0, 0, 0, 0);
@@ -880,14 +913,24 @@ int gather_counted(const void *h, const Shape &z, const long long *labels, long 
   auto *gmax = reinterpret_cast<uint32_t *>(ws + c.gmax);
   auto *lab = reinterpret_cast<long long *>(ws + c.labels);
   float *l = reinterpret_cast<float *>(ws + c.lse), *g = reinterpret_cast<float *>(ws + c.grad);
-  // the first of its chain: it waits for all before it
-  if (int rc = launch_chained(vocab_count_kernel, dim3(1), dim3(1024), 0, 1, false, s, labels,
-                              ignore, grad, z.T, place, count, gmax))
-    return rc;
-  if (int rc = launch_chained(vocab_gather_kernel<T>, dim3(z.T), dim3(128), 0, 1, true, s,
-                              static_cast<const T *>(h), z.ldh, z.D, z.T, place, count, labels,
-                              lse, grad, reinterpret_cast<T *>(ws + c.rows), lab, l, g))
-    return rc;
+  // the first of its chain waits for all before it.  Up to 1024 tokens every block of
+  // the gathering counts for itself, one launch less.
+  T *rows = reinterpret_cast<T *>(ws + c.rows);
+  const T *from = static_cast<const T *>(h);
+  if (z.T <= 1024) {
+    if (int rc = launch_chained(vocab_gather_kernel<T, true>, dim3(z.T), dim3(128), 0, 1, false, s,
+                                from, z.ldh, z.D, z.T, place, count, gmax, labels, ignore, lse,
+                                grad, rows, lab, l, g))
+      return rc;
+  } else {
+    if (int rc = launch_chained(vocab_count_kernel, dim3(1), dim3(1024), 0, 1, false, s, labels,
+                                ignore, grad, z.T, place, count, gmax))
+      return rc;
+    if (int rc = launch_chained(vocab_gather_kernel<T, false>, dim3(z.T), dim3(128), 0, 1, true, s,
+                                from, z.ldh, z.D, z.T, place, count, gmax, labels, ignore, lse,
+                                grad, rows, lab, l, g))
+      return rc;
+  }
   *tok = Counted{count, lab, l, g, gmax};
   return B2F_OK;
 }
