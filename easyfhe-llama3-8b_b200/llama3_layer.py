@@ -21,6 +21,12 @@ encrypted graph applies):
 * ``poly``:  the layer's own RMSNorm and SiLU Chebyshev approximations
   (evaluated in fp64) with exact softmax, which is what the encrypted graph
   approximates apart from its polynomial softmax and CKKS noise.
+
+Both run on the host in NumPy, or with ``device`` on the GPU (rotary positions
+by ``easyfhe.plain``, products by cuBLAS in fp64).  ``ClientHead`` is what the
+client does with a decrypted hidden state: its next token (4-bit head), its
+score against the prompt's tokens, the score's gradient; ``answer_check``
+compares the answer from the decrypted state with the plain one.
 """
 
 from __future__ import annotations
@@ -150,15 +156,185 @@ def mlp_delta_fp64(x2, weights, *, approximations=None) -> np.ndarray:
     return (act * (h2 @ f64(weights.up_proj).T)) @ f64(weights.down_proj).T
 
 
-def layer_fp64(hidden, weights, *, approximations=None, **kw) -> np.ndarray:
+def layer_fp64(hidden, weights, *, approximations=None, device=None, **kw) -> np.ndarray:
     """One Llama-3 decoder layer in fp64 (causal GQA with rotate-half RoPE,
     SwiGLU, RMSNorm with its gammas).  With ``approximations`` (the layer's
     LayerApproximations) RMSNorm's rsqrt and SiLU are its Chebyshev series;
-    softmax is always exact."""
+    softmax is always exact.  With ``device`` ("cuda") the layer runs there."""
 
+    if device is not None:
+        return _layer_fp64_device(hidden, weights, approximations, device, **kw)
     x = np.asarray(hidden, dtype=np.float64)
     x2 = x + attention_delta_fp64(x, weights, approximations=approximations, **kw)
     return x2 + mlp_delta_fp64(x2, weights, approximations=approximations)
+
+
+def _layer_fp64_device(hidden, weights, approximations, device, *, query_heads: int = 32,
+                       kv_heads: int = 8, head_dim: int = 128,
+                       rope_theta: float = 500000.0) -> np.ndarray:
+    """layer_fp64 on a GPU: the same formulas on fp64 tensors."""
+
+    import torch
+
+    from easyfhe import plain
+
+    def f64(a):
+        return torch.as_tensor(np.asarray(a)).to(device=device, dtype=torch.float64)
+
+    def chebyshev(x, entry):  # Clenshaw's recurrence, as chebyshev_fp64
+        lo, hi = (float(t) for t in entry["fit_interval"])
+        c = np.array(entry["coefficients"], dtype=np.float64)
+        c[0] *= 0.5
+        y = (2.0 * x - (lo + hi)) / (hi - lo)
+        b1 = b2 = torch.zeros_like(y)
+        for ck in c[:0:-1]:
+            b1, b2 = 2.0 * y * b1 - b2 + float(ck), b1
+        return y * b1 - b2 + float(c[0])
+
+    def norm(v, gamma, entry, eps=1e-5):
+        ms = (v * v).mean(dim=-1, keepdim=True)
+        scale = torch.rsqrt(ms + eps) if entry is None else chebyshev(ms, entry)
+        return v * scale * f64(gamma)
+
+    ap = approximations
+    with torch.no_grad():
+        x = f64(hidden)
+        seq = x.shape[0]
+        h = norm(x, weights.input_layernorm, None if ap is None else ap.input_norm)
+        q = (h @ f64(weights.q_proj).T).view(seq, query_heads, head_dim)
+        k = (h @ f64(weights.k_proj).T).view(seq, kv_heads, head_dim)
+        v = (h @ f64(weights.v_proj).T).view(seq, kv_heads, head_dim)
+        rope = plain.RopePlan(head_dim, theta=rope_theta, device=x.device)
+        q, k = plain.rope(q, k, positions=torch.arange(seq, device=x.device), plan=rope)
+        rep = query_heads // kv_heads
+        qh = q.transpose(0, 1)
+        kh, vh = (t.transpose(0, 1).repeat_interleave(rep, dim=0) for t in (k, v))
+        scores = qh @ kh.transpose(1, 2) / head_dim ** 0.5
+        ahead = torch.ones(seq, seq, dtype=torch.bool, device=x.device).triu(1)
+        p = torch.softmax(scores.masked_fill(ahead, float("-inf")), dim=-1)
+        x = x + (p @ vh).transpose(0, 1).reshape(seq, -1) @ f64(weights.o_proj).T
+        h = norm(x, weights.post_attention_layernorm,
+                 None if ap is None else ap.post_attention_norm)
+        g = h @ f64(weights.gate_proj).T
+        act = g / (1.0 + torch.exp(-g)) if ap is None else chebyshev(g, ap.silu)
+        x = x + (act * (h @ f64(weights.up_proj).T)) @ f64(weights.down_proj).T
+    return x.cpu().numpy()
+
+
+class ClientHead:
+    """The client's end of an encrypted prefill, on the GPU: final RMSNorm and
+    vocabulary head on decrypted hidden states (the reference's final_logits,
+    application/client.py:60-100).
+
+    The head is held twice: in bf16 for scores and gradients (``weight``,
+    [words, hidden]) and in 4 bits with a scale per ``group`` columns for the
+    next token, which is one row against the whole head."""
+
+    def __init__(self, gamma, lm_head, *, eps: float = 1e-5, group: int = 128,
+                 device: str = "cuda"):
+        import torch
+
+        self.gamma = torch.as_tensor(gamma).to(device=device, dtype=torch.float64)
+        self.weight = torch.as_tensor(lm_head).to(device=device, dtype=torch.bfloat16).contiguous()
+        if self.weight.dim() != 2 or self.gamma.shape != self.weight.shape[1:]:
+            raise ValueError(f"head of shape {tuple(self.weight.shape)} with norm weights "
+                             f"{tuple(self.gamma.shape)}")
+        self.eps, self.group = float(eps), int(group)
+        self.device = self.weight.device
+        self.quantize()
+
+    def quantize(self) -> None:
+        """Take the 4-bit head from ``weight`` again (after a training step)."""
+
+        from easyfhe import plain
+
+        self.four_bit = plain.quantize_q4(self.weight, group=self.group)
+
+    def norm(self, hidden):
+        """Final RMSNorm of hidden states [tokens, hidden], in fp64 on the device."""
+
+        import torch
+
+        x = torch.as_tensor(hidden).to(device=self.device, dtype=torch.float64)
+        return x * torch.rsqrt((x * x).mean(dim=-1, keepdim=True) + self.eps) * self.gamma
+
+    def next_logits(self, hidden):
+        """Logits [words] (float32) after the last of the hidden states, 4-bit head."""
+
+        from easyfhe import plain
+
+        return plain.q4_matvec(self.norm(hidden[-1:]).float(), self.four_bit)[0]
+
+    def next_token(self, hidden) -> int:
+        return int(self.next_logits(hidden).argmax())
+
+    def labels(self, tokens):
+        """What each position predicts: the next token; nothing for the last one."""
+
+        import torch
+
+        t = torch.as_tensor(tokens).to(device=self.device, dtype=torch.int64)
+        return torch.cat([t[1:], t.new_full((1,), -100)])
+
+    def score(self, hidden, tokens) -> float:
+        """Mean negative log-likelihood of the prompt's tokens under its hidden states."""
+
+        import torch
+
+        from easyfhe import plain
+
+        labels = self.labels(tokens)
+        loss, _ = plain.vocab_loss(self.norm(hidden).to(torch.bfloat16), self.weight, labels)
+        return float(loss.sum(dtype=torch.float64) / max(int((labels != -100).sum()), 1))
+
+    def gradient(self, hidden, tokens, *, need_weight: bool = True):
+        """(score, its gradient by the normed hidden states [tokens, hidden], by the
+        head [words, hidden] or None), gradients in bf16: what trains the head, the
+        one part of the model that the client holds in the clear, on decrypted
+        states, and what turns an error of those into a change of the score."""
+
+        import torch
+
+        from easyfhe import plain
+
+        labels = self.labels(tokens)
+        h = self.norm(hidden).to(torch.bfloat16)
+        count = max(int((labels != -100).sum()), 1)
+        loss, lse = plain.vocab_loss(h, self.weight, labels)
+        each = torch.full_like(loss, 1.0 / count)
+        dh, dw = plain.vocab_loss_grad(h, self.weight, labels, lse, each,
+                                       need_weight=need_weight)
+        return float(loss.sum(dtype=torch.float64) / count), dh, dw
+
+
+def synthetic_head(seed: int = 26081461, words: int = 128256, hidden: int = 4096, *,
+                   device: str = "cuda") -> ClientHead:
+    """A seeded head of Llama-3's size: N(0, 1 / hidden) words, gammas 1."""
+
+    import torch
+
+    gen = torch.Generator(device=device).manual_seed(int(seed))
+    w = torch.empty((words, hidden), dtype=torch.bfloat16, device=device)
+    for v0 in range(0, words, 16384):
+        part = w[v0:v0 + 16384]
+        part.copy_(torch.randn(part.shape, generator=gen, device=device) / hidden ** 0.5)
+    return ClientHead(torch.ones(hidden), w, device=device)
+
+
+def answer_check(decoded, reference, head: ClientHead, tokens) -> dict:
+    """How far the decryption error of hidden states moves the client's answer:
+    the prompt's score and next token from the decrypted and from the plain
+    states, and the score's change to first order in the error."""
+
+    import torch
+
+    score, dh, _ = head.gradient(reference, tokens, need_weight=False)
+    error = head.norm(decoded) - head.norm(reference)
+    a, b = head.next_logits(decoded), head.next_logits(reference)
+    return {"nll_decoded": head.score(decoded, tokens), "nll_plain": score,
+            "nll_change_first_order": float((error * dh.to(torch.float64)).sum()),
+            "next_token_decoded": int(a.argmax()), "next_token_plain": int(b.argmax()),
+            "logits_max_abs": float((a - b).abs().max())}
 
 
 def diff_stats(got: np.ndarray, want: np.ndarray) -> dict:
@@ -233,10 +409,14 @@ class ReferenceSession:
 
 
 def run_layer0(*, warmup: int = 1, repetitions: int = 1, seed: int = 26081461,
-               extra_args=(), check: bool = True) -> dict:
+               extra_args=(), check: bool = True, check_device=None,
+               head: ClientHead | None = None, tokens=None) -> dict:
     """Run ``runner.run`` of the reference's Layer-0 preset on this backend and
     return ``{"payload": <the reference's report>, "decoded": hidden [128, 4096],
-    "checks": {...}, "s_per_layer": ...}``."""
+    "checks": {...}, "s_per_layer": ...}``.  ``check_device`` ("cuda"): the fp64
+    layers run there.  With a ``head`` and the prompt's ``tokens`` the checks add
+    ``"answer"``, the client's answer from the decrypted layer against the plain
+    one."""
 
     import_reference()
     from llama3fhe.application import runner
@@ -259,11 +439,14 @@ def run_layer0(*, warmup: int = 1, repetitions: int = 1, seed: int = 26081461,
               "pack_stats": dict(fhe.PACK_STATS)}
     if check:
         hidden, weights, approx = synthetic_layer(seed)
+        exact = layer_fp64(hidden, weights, device=check_device)
         result["checks"] = {
-            "vs_fp64_exact": diff_stats(decoded, layer_fp64(hidden, weights)),
-            "vs_fp64_poly": diff_stats(decoded, layer_fp64(hidden, weights,
+            "vs_fp64_exact": diff_stats(decoded, exact),
+            "vs_fp64_poly": diff_stats(decoded, layer_fp64(hidden, weights, device=check_device,
                                                            approximations=approx)),
         }
+        if head is not None:
+            result["answer"] = answer_check(decoded, exact, head, tokens)
     return result
 
 
@@ -373,7 +556,8 @@ def tune_prefill_gains(num_layers: int = 32, seed: int = 26081461, log=print) ->
 
 
 def run_prefill(num_layers: int = 32, *, seed: int = 26081461, check: bool = True,
-                progress=None, diagnostic=None) -> dict:
+                progress=None, diagnostic=None, check_device=None,
+                head: ClientHead | None = None, tokens=None) -> dict:
     """An encrypted prefill of `num_layers` decoder layers through the reference's
     own model loop, unchanged, on this backend.
 
@@ -387,7 +571,8 @@ def run_prefill(num_layers: int = 32, *, seed: int = 26081461, check: bool = Tru
     synthetic layers (layer_weights) with each layer's own approximations into
     Llama3Model.forward (model.py:171-364): layer 0 consumes the encrypted
     input, every later layer refreshes the previous output inside its input
-    RMSNorm, and no boundary is decrypted until the end."""
+    RMSNorm, and no boundary is decrypted until the end.  ``check_device``,
+    ``head`` and ``tokens`` as in run_layer0."""
 
     import_reference()
     from llama3fhe import Llama3CKKSConfig
@@ -462,10 +647,12 @@ def run_prefill(num_layers: int = 32, *, seed: int = 26081461, check: bool = Tru
         exact = poly = np.asarray(hidden, np.float64)
         for i in range(n):
             w = layer_weights(i, seed)
-            exact = layer_fp64(exact, w)
-            poly = layer_fp64(poly, w, approximations=approx.for_layer(i))
+            exact = layer_fp64(exact, w, device=check_device)
+            poly = layer_fp64(poly, w, approximations=approx.for_layer(i), device=check_device)
         out["checks"] = {"vs_fp64_exact": diff_stats(decoded, exact),
                          "vs_fp64_poly": diff_stats(decoded, poly)}
+        if head is not None:
+            out["answer"] = answer_check(decoded, exact, head, tokens)
     return out
 
 
@@ -476,8 +663,14 @@ if __name__ == "__main__":
         GAINS_PATH.write_text(json.dumps(tune_prefill_gains(), indent=1) + "\n")
         sys.exit(0)
 
-    r = run_layer0()
+    extra = {}
+    if "--answer" in sys.argv[1:]:  # the client's answer too, on a seeded head and prompt
+        rng = np.random.default_rng(26081461)
+        extra = {"check_device": "cuda", "head": synthetic_head(),
+                 "tokens": rng.integers(0, 128256, 128)}
+    r = run_layer0(**extra)
     print(json.dumps({"s_per_layer": r["s_per_layer"], "checks": r.get("checks"),
+                      **({"answer": r["answer"]} if "answer" in r else {}),
                       "pack_stats": r["pack_stats"],
                       "performance": {k: v for k, v in r["payload"]["performance"].items()
                                       if k != "samples"}}, indent=1, default=str))

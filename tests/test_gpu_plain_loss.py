@@ -350,6 +350,25 @@ def test_refusals():
                                   need_hidden=need[0], need_weight=need[1])
 
 
+def test_a_small_workspace_is_refused():
+    from easyfhe import _native
+
+    h, w, labels, grad = _inputs(6, 40, 32, BF)
+    out = torch.full((4, 40, 32), 3.0, device="cuda")
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    args = (h.data_ptr(), 32, w.data_ptr(), 32, 3, 6, 40, 32, labels.data_ptr(), -100)
+    need = _native.lib.b2f_vocab_loss_workspace(6, 40, 32)
+    need_grad = _native.lib.b2f_vocab_loss_grad_workspace(6, 40, 32, 1)
+    with pytest.raises(ValueError, match="too small"):
+        _native.call("b2f_vocab_loss", *args, out[0].data_ptr(), out[1].data_ptr(),
+                     ws.data_ptr(), need - 1, None)
+    with pytest.raises(ValueError, match="too small"):
+        _native.call("b2f_vocab_loss_grad", *args, out[0].data_ptr(), out[1].data_ptr(),
+                     out[2].data_ptr(), out[3].data_ptr(), ws.data_ptr(), need_grad - 1, None)
+    torch.cuda.synchronize()
+    assert bool((out == 3.0).all())
+
+
 def test_no_wait_ran_out():
     from easyfhe import _native
 

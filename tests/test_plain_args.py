@@ -77,9 +77,9 @@ def test_q4_refusals():
 
 
 def test_vocab_loss_refusals():
-    def loss(match, h=P, ldh=64, ldw=64, dtype=3, t=4, v=9, d=64, ws=P, ws_bytes=1 << 20):
-        _refused("b2f_vocab_loss", h, ldh, P, ldw, dtype, t, v, d, P, -100, P, P, ws, ws_bytes,
-                 None, match=match)
+    def loss(match, h=P, ldh=64, ldw=64, dtype=3, t=4, v=9, d=64, ws=P):
+        _refused("b2f_vocab_loss", h, ldh, P, ldw, dtype, t, v, d, P, -100, P, P, ws,
+                 1 << 20, None, match=match)
 
     loss("dtype", dtype=1)
     loss("hidden size", d=60)
@@ -90,7 +90,6 @@ def test_vocab_loss_refusals():
     loss("null", ws=None)
     loss("misaligned", h=P + 8)
     loss("misaligned", ws=P + 16)
-    loss("too small", ws_bytes=16)
 
     def grad(match, dh=P, dw=P, lse=P):
         _refused("b2f_vocab_loss_grad", P, 64, P, 64, 3, 4, 9, 64, P, -100, lse, P, dh, dw, P, 0,
