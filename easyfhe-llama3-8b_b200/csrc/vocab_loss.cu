@@ -104,7 +104,8 @@ struct Tile {
   int m, n, split;
 };
 // Tokens run fastest, so that the blocks at work share W's rows; dW's rows (8 KB of a
-// 4096 wide head) are finished together: its columns run fastest.
+// 4096 wide head) are finished together: its columns run fastest.  dz starts from the
+// last words, which the forward pass has left in L2.
 template <int EPI>
 __device__ __forceinline__ Tile tile_at(const Tiles &t, int i) {
   Tile r;
@@ -112,6 +113,7 @@ __device__ __forceinline__ Tile tile_at(const Tiles &t, int i) {
     r.n = i % t.n_tiles, i /= t.n_tiles;
     r.m = i % t.m_tiles, r.split = i / t.m_tiles;
   } else {
+    if (EPI == EPI_DZ) i = t.total - 1 - i;
     r.m = i % t.m_tiles, i /= t.m_tiles;
     r.n = i % t.n_tiles, r.split = i / t.n_tiles;
   }
