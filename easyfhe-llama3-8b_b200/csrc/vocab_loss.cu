@@ -523,7 +523,8 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
         const bool live = t < M;
         const long long label = live ? a.tok.labels[t] : a.ignore;
         const long long at = label - a.n_first - n0;  // the label's column here
-        const int hit = at >= 0 && at < COLS && at < cols ? (int)at : -1;
+        // none past the last token: `ignore`, which stands in there, may be a word
+        const int hit = live && at >= 0 && at < COLS && at < cols ? (int)at : -1;
         float g = 0.0f, lse = 0.0f;
         if (EPI == EPI_DZ && live && label != a.ignore) {
           g = a.tok.grad[t] * scale;

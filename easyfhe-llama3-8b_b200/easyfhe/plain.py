@@ -146,7 +146,6 @@ class RopePlan:
         if dev.type != "cuda":
             raise ValueError("rope: libb200fhe runs on CUDA devices only (no CPU fallback)")
         self.freqs = torch.tensor(freqs, dtype=torch.float64, device=dev)
-        self.freqs_ptr = self.freqs.data_ptr()
         self.device, self.index = self.freqs.device, self.freqs.get_device()
 
 
@@ -211,7 +210,7 @@ def _rope(what, q, k, positions, plan, gradient):
         rc = lib.b2f_rope(a[0] if b is None else a[0] + b[0], 1 if b is None else 2,
                           _DTYPES[q.dtype], batch, seq, plan.head_dim, plan.rotary_dim,
                           plan.interleaved, positions.data_ptr(), wide,
-                          pos[0] if len(pos) == 2 else 0, pos[-1], plan.freqs_ptr, plan.factor,
+                          pos[0] if len(pos) == 2 else 0, pos[-1], plan.freqs.data_ptr(), plan.factor,
                           gradient, _raw_stream(plan.index))
         if rc:
             check(rc, what)
@@ -253,8 +252,7 @@ class Q4Weight:
         self.scale_dtype = scale_dtype
         self.zeros = bool(zeros)
         self.device, self.index = packed.device, packed.get_device()
-        self._args = (packed.data_ptr(), _DTYPES[scale_dtype], int(self.zeros), *self.shape,
-                      self.group)
+        self._args = (_DTYPES[scale_dtype], int(self.zeros), *self.shape, self.group)
 
     def nbytes(self) -> int:
         return self.packed.numel()
@@ -372,7 +370,8 @@ def q4_matvec(x: torch.Tensor, weight: Q4Weight, *,
         ld = x.stride(0) if rows > 1 else k
     y = x.new_empty((*shape[:-1], n), dtype=out_dtype)
     if rows:
-        rc = lib.b2f_q4_matvec(x.data_ptr(), code, ld, rows, *weight._args, y.data_ptr(),
+        rc = lib.b2f_q4_matvec(x.data_ptr(), code, ld, rows, weight.packed.data_ptr(),
+                               *weight._args, y.data_ptr(),
                                out_dtype is torch.float32, _raw_stream(weight.index))
         if rc:
             check(rc, "q4_matvec")
@@ -428,7 +427,7 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
     without the logits: (loss [tokens], lse [tokens]) in float32.
 
     hidden [tokens, D], weight [words, D] (both f16 or both bf16, D a multiple
-    of 8), labels int64.  A label of ignore_index gives 0 for both; any other
+    of 8; rows off 16-byte boundaries cost a copy), labels int64.  A label of ignore_index gives 0 for both; any other
     label outside the vocabulary gives a loss of NaN, as do logits that overflow."""
 
     index, t, v, d = _loss_args("vocab_loss", hidden, weight, labels)

@@ -121,3 +121,20 @@ def test_inference_mode_and_parameters():
     w.grad = dw
     torch.optim.SGD([w], lr=0.1).step()
     assert torch.isfinite(w).all()
+
+
+def test_copies_of_plans_and_weights_stand_alone():
+    import copy
+
+    from easyfhe import plain
+
+    plan = plain.RopePlan(64)
+    w = plain.quantize_q4(torch.randn((50, 128), device="cuda"))
+    q, x = torch.randn((4, 2, 64), device="cuda"), torch.randn((2, 128), device="cuda")
+    pos = torch.arange(4, device="cuda")
+    want = plain.rope(q, positions=pos, plan=plan), plain.q4_matvec(x, w)
+    plan2, w2 = copy.deepcopy(plan), copy.deepcopy(w)
+    plan.freqs.zero_()
+    w.packed.zero_()
+    assert torch.equal(plain.rope(q, positions=pos, plan=plan2), want[0])
+    assert torch.equal(plain.q4_matvec(x, w2), want[1])

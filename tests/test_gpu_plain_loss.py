@@ -143,6 +143,19 @@ def test_another_ignored_label(ignore):
     _check_grad(h, w, labels, grad, lse, ignore)
 
 
+@pytest.mark.parametrize("t", [1, 33, 129, 300, 1030])
+def test_ignored_label_is_a_word(t):
+    """Rows past the last token are no token's: with a word as the ignored label they
+    must leave no logit anywhere (many words: many entries beside the logits)."""
+    h, w, labels, grad = _inputs(t, 20011, 64, BF, ignored=0.0)
+    for ignore in (0, 7, 20010):
+        lab = labels.clone()
+        lab[lab == ignore] = 3
+        lab[::5] = ignore
+        _, lse = _check_loss(h, w, lab, ignore)
+        _check_grad(h, w, lab, grad, lse, ignore)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_garbage_in_ignored_rows_reaches_nothing(dtype):
     from easyfhe import plain
