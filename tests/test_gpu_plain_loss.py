@@ -123,6 +123,42 @@ def test_many_pieces_and_tiles(dtype, t, v, d):
     _check_grad(h, w, labels, grad, lse)
 
 
+def test_offsets_past_32_bits():
+    """A head of more than 2^31 values, labels among its first and last words."""
+    from easyfhe import plain
+
+    t, v, d = 7, 530000, 4096
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty((v, d), dtype=BF, device="cuda")
+    for v0 in range(0, v, 50000):
+        part = w[v0:v0 + 50000]
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda") / 64)
+    labels = torch.tensor([0, v - 1, v - 2, -100, 3, v // 2, v - 1], device="cuda")
+    h = (torch.randn((t, d), generator=g, device="cuda")
+         + 9 * w[labels.clamp(min=0)].float()).to(BF)
+    grad = torch.rand((t,), generator=g, device="cuda")
+    loss, lse = plain.vocab_loss(h, w, labels)
+    z = torch.cat([h.double() @ w[v0:v0 + 50000].double().T for v0 in range(0, v, 50000)], dim=1)
+    counted = labels != -100
+    want = torch.logsumexp(z, dim=1)
+    tol = (d / 16 + 2) * 2.0 ** -22 * float(z.abs().max()) + 2.0 ** -18 * float(want.max())
+    own = z.gather(1, labels.clamp(min=0)[:, None])[:, 0]
+    assert bool(((lse - want).abs() <= tol)[counted].all())
+    assert bool(((loss - (want - own)).abs() <= 2 * tol)[counted].all())
+    dh, dw = plain.vocab_loss_grad(h, w, labels, lse, grad)
+    dz = torch.exp(z - want[:, None])
+    dz[torch.arange(t), labels.clamp(min=0)] -= 1.0
+    dz *= torch.where(counted, grad, 0.0)[:, None]
+    ends = torch.cat([torch.arange(300), torch.arange(v - 300, v)]).cuda()
+    full = dz[:, ends].T @ h.double()
+    size = dz[:, ends].abs().T @ h.double().abs()
+    assert bool(((dw[ends] - full).abs() <= (2.1 * 2.0 ** -8 + 4 * tol) * size + 2.0 ** -126).all())
+    full = sum(dz[:, v0:v0 + 50000] @ w[v0:v0 + 50000].double() for v0 in range(0, v, 50000))
+    size = sum(dz[:, v0:v0 + 50000].abs() @ w[v0:v0 + 50000].double().abs()
+               for v0 in range(0, v, 50000))
+    assert bool(((dh - full).abs() <= (2.1 * 2.0 ** -8 + 4 * tol) * size).all())
+
+
 def test_every_token_ignored_and_none():
     h, w, labels, grad = _inputs(70, 400, 64, BF)
     none = torch.full_like(labels, -100)

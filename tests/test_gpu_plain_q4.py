@@ -195,6 +195,21 @@ def test_quantized_product_is_near_the_weight():
     _check(plain.q4_matvec(x, plain.quantize_q4(w)), x, codes, scales, zeros, 128)
 
 
+def test_offsets_past_32_bits():
+    """More than 2^32 codes: the last rows, in the last records, are the formula's."""
+    from easyfhe import plain
+
+    n, k = (1 << 20) + 21, 4096
+    g = torch.Generator(device="cuda").manual_seed(2)
+    codes = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.rand((n, 1), generator=g, device="cuda").half()
+    w = plain.pack_q4(codes, scales, group=k)
+    last = slice(n - 50, n)
+    for dtype, rows in ((torch.float32, 2), (torch.bfloat16, 9)):
+        x = _x(rows, k, dtype)
+        _check(plain.q4_matvec(x, w)[:, last], x, codes[last], scales[last], None, k)
+
+
 def test_capture_replays_on_new_rows():
     from easyfhe import plain
 
