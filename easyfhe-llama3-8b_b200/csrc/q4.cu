@@ -30,7 +30,7 @@
 // exact), each its own column of the product, and joined at the end.
 //
 // Up to four rows leave most of those 8 columns idle, and the conversion of the
-// nibbles is what bounds them (85 instructions a record, 70 us for one row against
+// nibbles is what bounds them (85 instructions a record, 58 us for one row against
 // 128256 x 4096, where HBM alone takes 41; as digits 47 instructions and 48 us).  They run on mma.sync m16n8k32 u8 x s8
 // instead: codes are bytes as they lie, two instructions for eight of them, and
 // x is a fixed-point number per row and 64 columns, X = round(x 2^sh) with the
@@ -53,7 +53,7 @@
 //
 // Measured: one binary32 row against 128256 x 4096, groups of 128: 48 us (5.6 TB/s, 86 %
 // of copy bandwidth); one bf16 row of 4096 x 4096: 6.0 us, where the launch, the set-up of
-// x and one trip to memory bound; 8 fp16 rows of 4096 x 14336 with zero points: 20 us,
+// x and one trip to memory bound; 8 fp16 rows of 4096 x 14336 with zero points: 17.5 us,
 // bound by the set-up (every block stages all 8 rows) and by 1.7 row blocks an SM.
 #include "plain.h"
 
@@ -385,7 +385,7 @@ constexpr int q4_batch(int nt) { return 4 / nt; }
 // How x enters the products: in its own type, split into three of bf16, or as
 // four digits of 8 bits.
 enum Q4Rows { Q4_SAME, Q4_SPLIT, Q4_DIGITS };
-constexpr int q4_max_warps(Q4Rows how) { return how == Q4_DIGITS ? 8 : 12; }
+constexpr int q4_max_warps(Q4Rows how) { return how == Q4_DIGITS ? 8 : 16; }
 // shared memory of one tile of x, of the digits with first sums and factors
 constexpr int q4_digit_bytes(int nt) { return 512 * nt; }
 constexpr int q4_tile_bytes(bool digits, bool g32, int nt, int cols) {
@@ -743,6 +743,8 @@ template <class T, Q4Rows HOW, int NT, bool ZERO, bool G32, bool SB>
 int launch_matvec(Q4Args a, int dev, int sms, cudaStream_t s) {
   constexpr int TPW = NT > 1 || G32 ? 4 : 8;
   constexpr bool INT = HOW == Q4_DIGITS;
+  B2F_CHECK_ARG(a.cols <= 8 * NT, "b2f_q4_matvec: %d columns of the product, %d fit", a.cols,
+                8 * NT);
   auto k = q4_matvec_kernel<T, HOW, NT, TPW, ZERO, G32, SB>;
   constexpr int most = q4_max_warps(HOW);
   static std::atomic<uint64_t> allowed{0};
@@ -806,17 +808,19 @@ int launch_cols(const Q4Args &a, bool zero, bool g32, bool sb, int dev, int sms,
   return sb ? launch_matvec<T, HOW, NT, false, false, true>(a, dev, sms, s)
             : launch_matvec<T, HOW, NT, false, false, false>(a, dev, sms, s);
 }
-// Binary32 rows (up to 4), or one or two rows of a 16-bit type, as digits where every
-// block has 4 (8) row blocks or more to spread their set-up over, else in their own type
-// or split.  One row of 4096 columns: binary32 12.1 against 13.8 us for 14336 weight
-// rows, 48 against 70 us for 128256, but 8.3 against 7.3 us for 4096; four binary32 rows
-// 84 against 110 us, four bf16 rows 84 against 76 us for 128256.
+// Up to four binary32 rows, or one or two of a 16-bit type, as digits where every block
+// has row blocks enough to spread their set-up over, else in their own type or split.
+// Digits against the other, us: one binary32 row of 4096 columns for 8192 weight rows 10.1
+// and 9.6, for 14336 12.1 and 13.1, for 128256 47.5 and 58.2; four 23.0 and 19.6 (14336),
+// 32.6 and 32.9 (32768), 84 and 107 (128256); one bf16 row 18.1 and 19.7 (32768), 48.0 and
+// 57.9 (128256), but three and four 79 and 60, 84 and 63.
 int launch_rows(Q4Args a, bool zero, bool g32, bool sb, int dev, int sms, cudaStream_t s) {
   using B = __nv_bfloat16;
   const int nt = a.rows <= 2 ? 1 : 2;
   const size_t digits = (size_t)((a.tiles_k + 7) / 8) * q4_tile_bytes(true, g32, nt, 0) + 49168;
   const int spread = (a.N + Q4_ROWS - 1) / Q4_ROWS / sms;
-  if ((a.dtype == B2F_F32 ? spread >= 4 : spread >= 8 && a.rows <= 2) && digits <= kQ4Smem) {
+  const bool wide = a.dtype == B2F_F32;
+  if (a.rows <= (wide ? 4 : 2) && spread >= (wide && a.rows <= 2 ? 6 : 12) && digits <= kQ4Smem) {
     a.cols = 4 * a.rows;
     return a.rows <= 2 ? launch_cols<B, Q4_DIGITS, 1>(a, zero, g32, sb, dev, sms, s)
                        : launch_cols<B, Q4_DIGITS, 2>(a, zero, g32, sb, dev, sms, s);
@@ -829,11 +833,9 @@ int launch_rows(Q4Args a, bool zero, bool g32, bool sb, int dev, int sms, cudaSt
   a.cols = a.rows;
   if (a.dtype == B2F_F16)
     return a.cols <= 8    ? launch_cols<__half, Q4_SAME, 1>(a, zero, g32, sb, dev, sms, s)
-           : a.cols <= 16 ? launch_cols<__half, Q4_SAME, 2>(a, zero, g32, sb, dev, sms, s)
-                          : launch_cols<__half, Q4_SAME, 4>(a, zero, g32, sb, dev, sms, s);
+                          : launch_cols<__half, Q4_SAME, 2>(a, zero, g32, sb, dev, sms, s);
   return a.cols <= 8    ? launch_cols<B, Q4_SAME, 1>(a, zero, g32, sb, dev, sms, s)
-         : a.cols <= 16 ? launch_cols<B, Q4_SAME, 2>(a, zero, g32, sb, dev, sms, s)
-                        : launch_cols<B, Q4_SAME, 4>(a, zero, g32, sb, dev, sms, s);
+                        : launch_cols<B, Q4_SAME, 2>(a, zero, g32, sb, dev, sms, s);
 }
 
 int check_shape(const char *who, int64_t N, int64_t K, int group) {
@@ -948,10 +950,17 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
   if (a.x_vec && esize == 2 && (uintptr_t)x % 16 == 0 && (rows == 1 || ldx % 8 == 0)) a.x_vec = 2;
   a.dtype = dtype;
   // rows in one pass: 4 of binary32 (8 rows of it as 24 columns took 217 us against
-  // 2 x 84), up to 32 of 16 bits, and no more than 8 blocks' shared memory holds of x
-  // (72 KB of each kept for the sums)
-  const long long fit = 8ll * (kQ4Smem - 72 * 1024) / (128ll * (a.tiles_k + 8));
-  const int step = (int)(dtype == B2F_F32 ? std::min(4ll, fit / 3) : std::min(32ll, fit));
+  // 2 x 84 for 128256 weight rows), up to 16 of 16 bits (17 as 32 columns: 190 us, 16 of them: 118), no more than 8 blocks' shared memory holds of x (72 KB
+  // of each kept for the sums), and of 16 bits no more than two hold unless that is less
+  // than 8 rows (16 rows of 14336 columns at once, on four: 44 us, as 8 and 8: 2 x 17);
+  // the passes share the rows out evenly
+  auto fit = [&](int blocks) {
+    return blocks * (long long)(kQ4Smem - 72 * 1024) / (128ll * (a.tiles_k + 8));
+  };
+  const long long most = dtype == B2F_F32 ? std::min(4ll, fit(8) / 3)
+                                          : std::min(16ll, std::max(fit(2), std::min(8ll, fit(8))));
+  const int64_t passes = (rows + most - 1) / most;
+  const int step = (int)((rows + passes - 1) / passes);
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     a.rows = (int)std::min<int64_t>(step, rows - r0);
     a.x = static_cast<const char *>(x) + r0 * ldx * esize;

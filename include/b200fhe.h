@@ -513,8 +513,8 @@ int b2f_q4_quantize(const void *w, int dtype, int64_t ld, int64_t N, int64_t K, 
 /* y[b][n] = sum_k weight[n][k] x[b][k] of up to 1024 rows of x (f32, f16 or
  * bf16, rows ldx apart), summed in binary32; y [rows][N] in x's type, or
  * binary32 with out_f32.  zeros: the packed weight has zero points.  The weight is
- * read once per 32 rows (4 of f32; fewer past about 4000 columns: what 8 blocks'
- * shared memory holds of x).  Binary32 rows and one or two rows of a 16-bit type may
+ * read once per 16 rows (4 of f32; fewer of long rows: what shared memory holds
+ * of x).  Binary32 rows and one or two rows of a 16-bit type may
  * be taken as fixed-point numbers, off by at most 2^-30 of the largest of their 64
  * columns; otherwise every value of x enters exactly. */
 int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const void *packed,
