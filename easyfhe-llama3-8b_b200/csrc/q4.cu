@@ -29,17 +29,17 @@
 // Rows in binary32 are split into three truncations to bf16 (8 + 8 + 8 bits:
 // exact), each its own column of the product, and joined at the end.
 //
-// Up to four rows leave most of those 8 columns idle, and the conversion of the
-// nibbles is what bounds them (85 instructions a record, 58 us for one row against
-// 128256 x 4096, where HBM alone takes 41; as digits 47 instructions and 48 us).  They run on mma.sync m16n8k32 u8 x s8
-// instead: codes are bytes as they lie, two instructions for eight of them, and
-// x is a fixed-point number per row and 64 columns, X = round(x 2^sh) with the
-// largest |X| in [2^29, 2^30], as four signed base-256 digits, each a column of
-// the product.  The sums code X are exact integers; the zero point enters as the
-// accumulator's first value, -z sum X, on top of 1.5 2^23, so that the sum's
-// bits read as binary32 are the sum plus that constant and no conversion is
-// needed.  X is off by at most 2^-30 of the largest of its 64 columns, which
-// binary32 accumulation of the same products is not better than.
+// Few rows leave most of those 8 columns idle, and the conversion of the nibbles is
+// what bounds them (85 instructions a record, 58 us for one row against 128256 x 4096,
+// where HBM alone takes 41; as digits 47 instructions and 48 us).  They run on mma.sync
+// m16n8k32 u8 x s8 instead: codes are bytes as they lie, two instructions for eight of
+// them, and x is a fixed-point number per row and 64 columns, X = round(x 2^sh) with
+// the largest |X| in [2^29, 2^30], as four signed base-256 digits, each a column of the
+// product.  The sums code X are exact integers; the zero point enters as the
+// accumulator's first value, -z sum X, on top of 1.5 2^23, so that the sum's bits read as
+// binary32 are the sum plus that constant and no conversion is needed.  X is off by at
+// most 2^-30 of the largest of its 64 columns, which binary32 accumulation of the same
+// products is not better than.
 //
 // A block takes row blocks in turn, its warps chunks of a few records along the
 // columns (and, where those are few, several row blocks at once).  x is laid out in
@@ -949,11 +949,12 @@ int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const voi
   a.x_vec = (uintptr_t)x % (4 * esize) == 0 && (rows == 1 || ldx % 4 == 0);
   if (a.x_vec && esize == 2 && (uintptr_t)x % 16 == 0 && (rows == 1 || ldx % 8 == 0)) a.x_vec = 2;
   a.dtype = dtype;
-  // rows in one pass: 4 of binary32 (8 rows of it as 24 columns took 217 us against
-  // 2 x 84 for 128256 weight rows), up to 16 of 16 bits (17 as 32 columns: 190 us, 16 of them: 118), no more than 8 blocks' shared memory holds of x (72 KB
-  // of each kept for the sums), and of 16 bits no more than two hold unless that is less
-  // than 8 rows (16 rows of 14336 columns at once, on four: 44 us, as 8 and 8: 2 x 17);
-  // the passes share the rows out evenly
+  // rows in one pass: 4 of binary32 (8 of them as 24 columns took 217 us against 2 x 84
+  // for 128256 weight rows), up to 16 of 16 bits (17 as 32 columns: 190 us, 16 of them:
+  // 118), no more than 8 blocks' shared memory holds of x (72 KB of each kept for the
+  // sums), and of 16 bits no more than two hold unless that is less than 8 rows (16 rows of
+  // 14336 columns at once, on four blocks: 44 us, as 8 and 8: 2 x 17); the passes share the
+  // rows out evenly
   auto fit = [&](int blocks) {
     return blocks * (long long)(kQ4Smem - 72 * 1024) / (128ll * (a.tiles_k + 8));
   };

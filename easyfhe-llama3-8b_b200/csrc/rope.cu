@@ -18,10 +18,11 @@
 // loads of a head before anything else of it (131 us with the second one after the
 // output's address), and registers for five blocks of 256 threads on an SM (four
 // with two heads in flight per thread: 129 us).
-// The angle of a far position needs more than binary32: p f is formed in binary64 and reduced there to a fraction of a turn in [-1/2,
-// 1/2], whose sine and cosine are then taken in binary32 (the reduction's
-// error is 2^-52 of the turns, the rounding of the fraction 2^-25 of a turn);
-// binary64 inputs take binary64 sines of p f.
+// The angle of a far position needs more than binary32: p f is formed in binary64
+// and reduced there to a fraction of a turn in [-1/2, 1/2], whose sine and cosine
+// are then taken in binary32 (the reduction's error is 2^-52 of the turns, the
+// rounding of the fraction 2^-25 of a turn); binary64 inputs take binary64 sines of
+// p f.
 #include "plain.h"
 
 #include <cuda_bf16.h>
@@ -230,7 +231,8 @@ int launch_rope(RopeArgs a, int parts, int sms, cudaStream_t s) {
   const int by = std::min((a.heads + passes - 1) / passes, ROPE_THREADS / bx);
   const dim3 block(bx, by);
   // few tokens: one to a block; more share a block's pipeline
-  a.block_tokens = (int)std::max<long long>(1, std::min<long long>(ROPE_TOKENS, a.batch * a.seq / (8 * sms)));
+  a.block_tokens = (int)std::max<long long>(
+      1, std::min<long long>(ROPE_TOKENS, a.batch * a.seq / (8 * sms)));
   const dim3 grid((unsigned)((a.seq + a.block_tokens - 1) / a.block_tokens),
                   (unsigned)std::min<long long>(a.batch, 65535));
   const size_t smem = (size_t)a.block_tokens * half * 2 * sizeof(typename Wide<T>::V);

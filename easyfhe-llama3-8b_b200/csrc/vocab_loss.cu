@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(512)
   sm[threadIdx.y][threadIdx.x] = make_float2(m, s);
   __syncthreads();
   if (threadIdx.y >= 8) return;
-  for (int y = threadIdx.y + 8; y < 64; y += 8) join(m, s, sm[y][threadIdx.x].x, sm[y][threadIdx.x].y);
+  for (int y = threadIdx.y + 8; y < 64; y += 8)
+    join(m, s, sm[y][threadIdx.x].x, sm[y][threadIdx.x].y);
   sm[threadIdx.y][threadIdx.x] = make_float2(m, s);
   asm volatile("bar.sync 1, 64;\n" ::: "memory");
   if (threadIdx.y || t >= T) return;
@@ -706,7 +707,8 @@ __global__ void __launch_bounds__(1024)
       const int u = __shfl_up_sync(~0u, v, o);
       if (lane >= o) v += u;
     }
-    const int mine = before + __shfl_sync(~0u, v, warp) - __popc(mask) + __popc(mask & ((1u << lane) - 1));
+    const int warps_before = __shfl_sync(~0u, v, warp) - __popc(mask);
+    const int mine = before + warps_before + __popc(mask & ((1u << lane) - 1));
     before += __shfl_sync(~0u, v, 31);
     if (t < T) place[t] = in ? mine : -1;
     __syncthreads();
@@ -919,7 +921,8 @@ template <class T>
 int gather_counted(const void *h, const Shape &z, const long long *labels, long long ignore,
                    const float *lse, const float *grad, char *ws, const CountedSpace &c,
                    Counted *tok, cudaStream_t s) {
-  int *place = reinterpret_cast<int *>(ws + c.place), *count = reinterpret_cast<int *>(ws + c.count);
+  int *place = reinterpret_cast<int *>(ws + c.place);
+  int *count = reinterpret_cast<int *>(ws + c.count);
   auto *gmax = reinterpret_cast<uint32_t *>(ws + c.gmax);
   auto *lab = reinterpret_cast<long long *>(ws + c.labels);
   float *l = reinterpret_cast<float *>(ws + c.lse), *g = reinterpret_cast<float *>(ws + c.grad);
@@ -1068,7 +1071,8 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
     a.n_first = v0;
     a.tok = tok, a.ignore = ignore, a.vocab = z.V;
     if (int rc = encode_map<T>(&dz_out, dz, z.T, words, p.piece, 32)) return rc;
-    if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, dz_out, a, group, true, dev, sms, s))
+    if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, dz_out, a, group, true, dev, sms,
+                                                      s))
       return rc;
     if (dh) {
       if (int rc = encode_map<T>(&dz_k, dz, z.T, words, p.piece, VL_M)) return rc;
@@ -1077,8 +1081,8 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
       b.k_first = v0;
       b.tok = tok;
       b.accumulate = i > 0;
-      if (int rc = launch_gemm<T, EPI_PARTIAL, false, true>(dz_k, w_n, sums, b, group, true, dev, sms,
-                                                         s))
+      if (int rc = launch_gemm<T, EPI_PARTIAL, false, true>(dz_k, w_n, sums, b, group, true, dev,
+                                                            sms, s))
         return rc;
     }
     if (dw) {

@@ -210,8 +210,8 @@ def _rope(what, q, k, positions, plan, gradient):
         rc = lib.b2f_rope(a[0] if b is None else a[0] + b[0], 1 if b is None else 2,
                           _DTYPES[q.dtype], batch, seq, plan.head_dim, plan.rotary_dim,
                           plan.interleaved, positions.data_ptr(), wide,
-                          pos[0] if len(pos) == 2 else 0, pos[-1], plan.freqs.data_ptr(), plan.factor,
-                          gradient, _raw_stream(plan.index))
+                          pos[0] if len(pos) == 2 else 0, pos[-1], plan.freqs.data_ptr(),
+                          plan.factor, gradient, _raw_stream(plan.index))
         if rc:
             check(rc, what)
     return a[1] if b is None else (a[1], b[1])
@@ -427,8 +427,9 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
     without the logits: (loss [tokens], lse [tokens]) in float32.
 
     hidden [tokens, D], weight [words, D] (both f16 or both bf16, D a multiple
-    of 8; rows off 16-byte boundaries cost a copy), labels int64.  A label of ignore_index gives 0 for both; any other
-    label outside the vocabulary gives a loss of NaN, as do logits that overflow."""
+    of 8; rows off 16-byte boundaries cost a copy), labels int64.  A label of
+    ignore_index gives 0 for both; any other label outside the vocabulary gives a
+    loss of NaN, as do logits that overflow."""
 
     index, t, v, d = _loss_args("vocab_loss", hidden, weight, labels)
     if _current_device() != index:

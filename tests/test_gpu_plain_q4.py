@@ -59,8 +59,8 @@ def _check(y, x, codes, scales, zeros, group):
     (300, 4096, 128, False, torch.bfloat16), (64, 14336, 64, True, torch.float16),
     (2500, 576, 192, True, torch.bfloat16), (28500, 200, 64, True, torch.bfloat16),
     (30005, 300, 32, False, torch.float16), (29999, 640, 32, True, torch.bfloat16),
-    (20000, 1100, 128, False, torch.bfloat16), (30001, 300, 64, True, torch.float16), (18, 70001, 128, False, torch.float16),
-    (33, 131072, 32, True, torch.bfloat16)])
+    (20000, 1100, 128, False, torch.bfloat16), (30001, 300, 64, True, torch.float16),
+    (18, 70001, 128, False, torch.float16), (33, 131072, 32, True, torch.bfloat16)])
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 8, 11, 33])
 def test_matvec(dtype, n, k, group, zeros, scale, rows):
     from easyfhe import plain
