@@ -1077,7 +1077,11 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
     if (dh) {
       if (int rc = encode_map<T>(&dz_k, dz, z.T, words, p.piece, VL_M)) return rc;
       VocabArgs b{};
-      b.M = z.T, b.N = z.D, b.K = words, b.splits = p.splits;
+      b.M = z.T, b.N = z.D, b.K = words;
+      // the last piece may have too few words for all the splits; one without a K block
+      // would add what its accumulator held before
+      const int kb = (words + VL_K - 1) / VL_K, per = (kb + p.splits - 1) / p.splits;
+      b.splits = (kb + per - 1) / per;
       b.k_first = v0;
       b.tok = tok;
       b.accumulate = i > 0;

@@ -123,6 +123,21 @@ def test_many_pieces_and_tiles(dtype, t, v, d):
     _check_grad(h, w, labels, grad, lse)
 
 
+def test_a_last_piece_of_fewer_words():
+    """Many tokens over a vocabulary whose last piece holds 64 words: fewer K blocks than
+    the sum over a full piece is split into."""
+
+    h, w, labels, grad = _inputs(38400, 49984, 64, BF, ignored=0.992)
+    from easyfhe import plain
+
+    _, lse = plain.vocab_loss(h, w, labels)
+    dh, _ = plain.vocab_loss_grad(h, w, labels, lse, grad, need_weight=False)
+    kept = labels != -100
+    assert 200 < int(kept.sum()) < 400 and not dh[~kept].any()
+    _check_grad(h[kept], w, labels[kept], grad[kept], lse[kept], need=(True, False),
+                got=(dh[kept], None))
+
+
 def test_offsets_past_32_bits():
     """A head of more than 2^31 values, labels among its first and last words."""
     from easyfhe import plain
