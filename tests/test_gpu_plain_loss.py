@@ -276,6 +276,51 @@ def test_confident_and_hopeless_tokens(dtype):
     _check_grad(h, w, labels, grad, lse)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("v", [3, 300, 5000])
+def test_a_small_loss_keeps_its_precision(dtype, v):
+    """Losses down to 1e-9.  The others' share of the sum is exp(z_v - z_label), each off by
+    2 e relative with e a logit's error (D / 16 + 2 accumulations of 2^-22 max|z|), the
+    exponential's argument (its own step, 2^-23 of up to 64) and the sums: 32 terms a group
+    and at most 100 joins of three roundings, 2^-24 each."""
+    from easyfhe import plain
+
+    h, w, labels, _ = _inputs(40, v, 64, dtype, ignored=0.0)
+    lean = torch.linspace(0, 32, 40, device="cuda")[:, None]
+    h = (0.2 * h.float() + lean * w[labels].float()).to(dtype)
+    loss, _ = plain.vocab_loss(h, w, labels)
+    z = h.double() @ w.double().T
+    own = z.gather(1, labels[:, None])
+    others = torch.exp(z - own).scatter(1, labels[:, None], 0.0).sum(1)
+    want = torch.log1p(others)
+    e = (64 / 16 + 2) * 2.0 ** -22 * float(z.abs().max())
+    tol = want * (2 * e + 64 * 2.0 ** -22 + (32 + 300) * 2.0 ** -24)
+    small = (z - own).max(1).values <= 0  # the label's word is the likeliest
+    assert int(small.sum()) > 20 and float(want[small].min()) < 1e-6
+    assert bool(((loss.double() - want).abs() <= tol)[small].all()), float(
+        ((loss.double() - want).abs() / tol)[small].max())
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t", [3, 200])
+def test_long_sums_of_one_sign(dtype, t):
+    """8192 positive products: an accumulation over all of them would lose up to 512 steps of
+    the sum.  Chunks of 512 products lose 32 steps (2^-23) of their own sums, which add up to
+    the logit, and 16 half steps where they are joined; lse and loss have 16 steps besides."""
+    from easyfhe import plain
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h = (0.5 + torch.rand((t, 8192), generator=g, device="cuda")).to(dtype)
+    w = ((0.5 + torch.rand((700, 8192), generator=g, device="cuda")) / 200).to(dtype)
+    labels = torch.randint(0, 700, (t,), generator=g, device="cuda")
+    loss, lse = plain.vocab_loss(h, w, labels)
+    want, want_lse, z = loss64(h, w, labels, -100)
+    tol = (34 * 2.0 ** -23 + 16 * 2.0 ** -24 + 16 * 2.0 ** -23) * float(z.abs().max())
+    assert bool(((lse.double() - want_lse).abs() <= tol).all()), float(
+        (lse.double() - want_lse).abs().max() / tol)
+    assert bool(((loss.double() - want).abs() <= 2 * tol).all())
+
+
 def test_gradients_span_types_ranges():
     """Upstream gradients from 1e-8 to 1e4 in fp16: the scale keeps what the
     outputs can hold, and zeros give zeros."""
