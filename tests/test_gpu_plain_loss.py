@@ -123,6 +123,40 @@ def test_many_pieces_and_tiles(dtype, t, v, d):
     _check_grad(h, w, labels, grad, lse)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,v,d", [(1, 300, 8), (2, 700, 64), (31, 1003, 200), (33, 500, 72),
+                                   (64, 2000, 136)])
+def test_few_tokens_lose_nothing_but_the_outputs_rounding(dtype, t, v, d):
+    """dz in two parts: off by the square of half a step instead of half a step.  An output
+    may differ from its value by its own half step, the steps of its sum (2^-22 of the terms
+    for each accumulation), dz's p (2 e, and 2^-20 for the exponential and its argument),
+    what the second part cannot hold, and fp16's subnormals (2^-25 and, of dz under its
+    scale, 2^-38 max|g|)."""
+    from easyfhe import plain
+
+    h, w, labels, grad = _inputs(t, v, d, dtype, ignored=0.2 if t > 2 else 0.0)
+    _, lse = plain.vocab_loss(h, w, labels)
+    dh, dw = plain.vocab_loss_grad(h, w, labels, lse, grad)
+    dz = loss_grad64(h, w, labels, -100, grad)
+    _, want_lse, e = _errors(h, w, labels, -100)
+    counted = labels != -100
+    g = torch.where(counted, grad.double().abs(), 0.0)[:, None]
+    p = torch.exp(h.double() @ w.double().T - want_lse[:, None])
+    step = half_step(dtype)
+    size = dz.abs() * (2 * step ** 2 + 2.0 ** -20) + 2 * e[:, None] * p * g + 2.0 ** -126
+    if dtype == FP:
+        size = size + 2.0 ** -38 * float(g.max()) * counted[:, None]
+    hc = torch.where(counted[:, None], h.double(), 0.0)
+    for got, want, tol, n, total in (
+            (dh, dz @ w.double(), size @ w.double().abs(), v, dz.abs() @ w.double().abs()),
+            (dw, dz.T @ hc, size.T @ hc.abs(), 128, dz.abs().T @ hc.abs())):
+        tol = tol + (n / 16 + 16) * 2.0 ** -22 * total + 1.01 * step * want.abs() + 2.0 ** -126
+        if dtype == FP:
+            tol = tol + 2.0 ** -25
+        diff = (got.double() - want).abs()
+        assert bool((diff <= tol).all()), float((diff / tol).max())
+
+
 def test_a_last_piece_of_fewer_words():
     """Many tokens over a vocabulary whose last piece holds 64 words: fewer K blocks than
     the sum over a full piece is split into."""
