@@ -35,10 +35,10 @@
 // there dz is scaled by a power of two that brings the largest |g| to 2^14 and
 // the products are scaled back in binary32.
 //
-// Measured on a 128256 x 4096 head in bf16: the score of 128 tokens 172-180 us (W read
-// once at 89-93 % of copy bandwidth); a training step on them 870 us = that + 182 (dz:
+// Measured on a 128256 x 4096 head in bf16: the score of 128 tokens 174-181 us (W read
+// once at 88-92 % of copy bandwidth); a training step on them 870 us = that + 182 (dz:
 // W again) + 155 (dh: W a third time) + 284 (dW; clearing as many bytes takes 275); a
-// step on 4096 tokens 12.4 ms, 1.25 PFLOP/s over the four products of the counted
+// step on 4096 tokens 12.4-13.1 ms, 1.19-1.25 PFLOP/s over the four products of the counted
 // tokens, under the power cap (cuBLAS sustains 1.385).  dh, dW and the next piece's logits
 // side by side on clusters of their own were no faster (672 against 660 us).
 #include <cuda.h>
