@@ -31,9 +31,9 @@
 // dz is rounded to the operand type before its two products (once from 65 tokens
 // on: relative to each dz at most half a step of the type, the size of the rounding of
 // the gradients themselves; in two parts below, VL_LOW), and formed from p - 1 (expm1)
-// at the label, where lse's own rounding is all that a confident token loses.  fp16 cannot hold g p of a rare word, so
-// there dz is scaled by a power of two that brings the largest |g| to 2^14 and
-// the products are scaled back in binary32.
+// at the label, where lse's own rounding is all that a confident token loses.  fp16
+// cannot hold g p of a rare word, so there dz is scaled by a power of two that brings
+// the largest |g| to 2^14 and the products are scaled back in binary32.
 //
 // Measured on a 128256 x 4096 head in bf16: the score of 128 tokens 174-181 us (W read
 // once at 88-92 % of copy bandwidth); a training step on them 870 us = that + 182 (dz:
