@@ -30,10 +30,11 @@
 //
 // dz is rounded to the operand type before its two products (once from 65 tokens
 // on: relative to each dz at most half a step of the type, the size of the rounding of
-// the gradients themselves; in two parts below, VL_LOW), and formed from p - 1 (expm1)
-// at the label, where lse's own rounding is all that a confident token loses.  fp16
-// cannot hold g p of a rare word, so there dz is scaled by a power of two that brings
-// the largest |g| to 2^14 and the products are scaled back in binary32.
+// the gradients themselves; what it leaves at the label joins dh in binary32, where it
+// would be shared by a token's whole row.  In two parts below, VL_LOW), and formed from
+// p - 1 (expm1) at the label, where lse's own rounding is all that a confident token
+// loses.  fp16 cannot hold g p of a rare word, so there dz is scaled by a power of two
+// that brings the largest |g| to 2^14 and the products are scaled back in binary32.
 //
 // Measured on a 128256 x 4096 head in bf16: the score of 128 tokens 174-181 us (W read
 // once at 88-92 % of copy bandwidth); a training step on them 870 us = that + 182 (dz:
@@ -118,6 +119,7 @@ struct VocabArgs {
   int vocab;
   float2 *part;       // [slots][M] (max, rest)
   float *label_logit; // [M]
+  float *label_left;  // [M] what rounding left of dz at the label
   int accumulate;     // dh: add to the partial sums
 };
 
@@ -336,6 +338,14 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  else
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
 // power of two S with S max|g| in [2^13, 2^14] (1 for a zero, infinite or NaN
@@ -651,6 +661,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
                 if (j == h) v[j] = own;
               }
               put_half<T>(sl, lane, q, v);
+              if (!two && h >= 0 && h < 32) a.label_left[t] = left_over<T>(own);
             }
             filled();
             if (lane == 0 && m0 + quarter * 32 < (two ? VL_LOW : a.M)) {
@@ -889,12 +900,15 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-// Sum of the splits' dh, rounded once; zero rows for ignored tokens.  Four threads share
+// Sum of the splits' dh and of what rounding left of dz at the label (one row of W a
+// token), rounded once; zero rows for ignored tokens.  Four threads share
 // the splits of four columns, and their sums are added in order.
 template <class T>
 __global__ void __launch_bounds__(256)
     vocab_sum_kernel(const float4 *__restrict__ partial, int splits, int tokens, int low, int d4,
                      const int *__restrict__ place, const uint32_t *__restrict__ grad_max,
+                     const long long *__restrict__ labels, const float *__restrict__ label_left,
+                     const T *__restrict__ w, long long ldw, int vocab,
                      uint2 *__restrict__ out) {
   __shared__ float4 sm[3][64];
   let_next_start();
@@ -918,6 +932,13 @@ __global__ void __launch_bounds__(256)
   __syncthreads();
   if (y || i >= n) return;
   for (int k = 0; k < 3; ++k) add(sm[k][x]);
+  if (!low && p >= 0 && labels[p] >= 0 && labels[p] < vocab) {
+    const uint2 row = *reinterpret_cast<const uint2 *>(w + labels[p] * ldw + 4 * c);
+    const float left = label_left[p];
+    const float2 a = unpack2<T>(row.x), b = unpack2<T>(row.y);
+    v.x = fmaf(left, a.x, v.x), v.y = fmaf(left, a.y, v.y);
+    v.z = fmaf(left, b.x, v.z), v.w = fmaf(left, b.y, v.w);
+  }
   float scale = 1.0f;
   if constexpr (std::is_same<T, __half>::value) scale = 1.0f / dz_scale(grad_max);
   out[i] = make_uint2(pack2<T>(v.x * scale, v.y * scale), pack2<T>(v.z * scale, v.w * scale));
@@ -1008,7 +1029,7 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // The counted tokens' place in a workspace.
 struct CountedSpace {
-  size_t place, count, gmax, labels, lse, grad, rows, end;
+  size_t place, count, gmax, labels, lse, grad, left, rows, end;
 };
 CountedSpace counted_space(int64_t T, int64_t D, bool grad) {
   CountedSpace c{};
@@ -1020,6 +1041,7 @@ CountedSpace counted_space(int64_t T, int64_t D, bool grad) {
   };
   c.place = take(T * 4), c.count = take(4), c.gmax = take(4), c.labels = take(T * 8);
   c.lse = take(grad ? T * 4 : 0), c.grad = take(grad ? T * 4 : 0);
+  c.left = take(grad ? T * 4 : 0);
   c.rows = take((size_t)T * D * 2);
   c.end = off;
   return c;
@@ -1163,6 +1185,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
              const Plan &p, char *ws, int dev, int sms, cudaStream_t s) {
   T *hc = reinterpret_cast<T *>(ws + p.c.rows), *dz = reinterpret_cast<T *>(ws + p.dz);
   float *partial = reinterpret_cast<float *>(ws + p.partial);
+  float *left = reinterpret_cast<float *>(ws + p.c.left);
   Counted tok;
   if (int rc = gather_counted<T>(h, z, labels, ignore, lse, grad, ws, p.c, &tok, s)) return rc;
   const int group = blocks_per_tile(z.T);
@@ -1182,6 +1205,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
     a.M = z.T, a.N = words, a.K = z.D, a.splits = 1;
     a.n_first = v0;
     a.tok = tok, a.ignore = ignore, a.vocab = z.V, a.low = low;
+    a.label_left = left;
     if (int rc = encode_map<T>(&dz_out, dz, rows, words, p.piece, 32)) return rc;
     if (int rc = launch_gemm<T, EPI_DZ, false, false>(h_k, w_k, dz_out, a, group, true, dev, sms,
                                                       s))
@@ -1216,6 +1240,7 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
     return launch_chained(vocab_sum_kernel<T>, dim3((unsigned)((n4 + 63) / 64)), dim3(256), 0, 1,
                           true, s, reinterpret_cast<const float4 *>(partial), p.splits, z.T,
                           low, z.D / 4, reinterpret_cast<const int *>(ws + p.c.place), tok.grad_max,
+                          tok.labels, left, static_cast<const T *>(w), z.ldw, z.V,
                           static_cast<uint2 *>(dh));
   }
   return B2F_OK;

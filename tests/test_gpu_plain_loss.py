@@ -157,6 +157,36 @@ def test_few_tokens_lose_nothing_but_the_outputs_rounding(dtype, t, v, d):
         assert bool((diff <= tol).all()), float((diff / tol).max())
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,v,d", [(65, 300, 64), (130, 2000, 200), (1100, 700, 72)])
+def test_hidden_gradient_keeps_the_labels_dz(dtype, t, v, d):
+    """dz is rounded by up to half a step at every word but the label, whose remainder is
+    added in binary32: there only half a step squared is lost (2^-24 of it).  The rest as for
+    few tokens."""
+    from easyfhe import plain
+
+    h, w, labels, grad = _inputs(t, v, d, dtype, ignored=0.2)
+    _, lse = plain.vocab_loss(h, w, labels)
+    dh, _ = plain.vocab_loss_grad(h, w, labels, lse, grad, need_weight=False)
+    dz = loss_grad64(h, w, labels, -100, grad)
+    _, want_lse, e = _errors(h, w, labels, -100)
+    counted = labels != -100
+    g = torch.where(counted, grad.double().abs(), 0.0)[:, None]
+    p = torch.exp(h.double() @ w.double().T - want_lse[:, None])
+    step = half_step(dtype)
+    lost = torch.full_like(dz, step)
+    lost[torch.arange(t), labels.clamp(min=0)] = 2.0 ** -24
+    size = dz.abs() * (1.01 * lost + 2.0 ** -20) + 2 * e[:, None] * p * g + 2.0 ** -126
+    if dtype == FP:
+        size = size + 2.0 ** -38 * float(g.max()) * counted[:, None]
+    want, total = dz @ w.double(), dz.abs() @ w.double().abs()
+    tol = size @ w.double().abs() + (v / 16 + 16) * 2.0 ** -22 * total
+    tol = tol + 1.01 * step * want.abs() + 2.0 ** -126 + (2.0 ** -25 if dtype == FP else 0.0)
+    diff = (dh.double() - want).abs()
+    assert bool((diff <= tol).all()), float((diff / tol).max())
+    assert not dh[~counted].any()
+
+
 def test_a_last_piece_of_fewer_words():
     """Many tokens over a vocabulary whose last piece holds 64 words: fewer K blocks than
     the sum over a full piece is split into."""
