@@ -30,8 +30,9 @@
 //
 // dz is rounded to the operand type before its two products (once from 65 tokens
 // on: relative to each dz at most half a step of the type, the size of the rounding of
-// the gradients themselves; what it leaves at the label joins dh in binary32, where it
-// would be shared by a token's whole row.  In two parts below, VL_LOW), and formed from
+// the gradients themselves; what it leaves at the label joins dh and dW in binary32: it
+// is shared by a token's whole row of dh, and a word that a token has as its label owes
+// nearly all of its row of dW to that.  In two parts below, VL_LOW), and formed from
 // p - 1 (expm1) at the label, where lse's own rounding is all that a confident token
 // loses.  fp16 cannot hold g p of a rare word, so there dz is scaled by a power of two
 // that brings the largest |g| to 2^14 and the products are scaled back in binary32.
@@ -98,12 +99,24 @@ enum Epilogue { EPI_STATS, EPI_DZ, EPI_PARTIAL, EPI_OUT };
 // all is latency; more tokens' dz would take a second tile and both products' time again.
 constexpr int VL_LOW = 64;
 
+// The counted tokens in the order of their labels (those of one label in their own), so
+// that dW finds the tokens of its words: first[g] is the place of the first one whose label
+// is 32 g or more, for g from 0 to the groups' number inclusive.  Labels outside the
+// vocabulary count as its size, behind all words.
+constexpr int VL_GROUP = 32;  // words that a warp of dW's epilogue holds
+struct ByLabel {
+  int *token, *label, *first;  // null: not wanted
+  int groups;
+};
+
 // Tokens as the products see them: `rows` of the workspace, the counted ones first.
 struct Counted {
   const int *count;          // how many; null: all of them
   const long long *labels;   // of the counted tokens
   const float *lse, *grad;
   const uint32_t *grad_max;  // bits of max |g| (fp16)
+  const void *rows;          // [.][D]
+  ByLabel by;
 };
 
 struct VocabArgs {
@@ -714,19 +727,80 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
         }
         release();
       } else {
-        if (sums && !ready()) break;
-        const uint32_t acc = accumulator();
-        for (int c = 0; c < COLS && c < cols; c += 64) {
+        // the tokens whose label is one of this warp's words, the first 32 of them in its
+        // lanes: asked for before the wait
+        const int word0 = a.m_first + m0 + quarter * 32;
+        int own = 0, own_end = 0, own_token = 0, own_label = 0;
+        float own_left = 0.0f;
+        if (sums && a.tok.by.first) {
+          own = a.tok.by.first[word0 / VL_GROUP], own_end = a.tok.by.first[word0 / VL_GROUP + 1];
+          if (own + lane < own_end) {
+            own_token = a.tok.by.token[own + lane], own_label = a.tok.by.label[own + lane];
+            own_left = a.label_left[own_token];
+          }
+        }
+        float z[COLS / 32][32];
+        if (sums) {
+          if (!ready()) break;
+          const uint32_t acc = accumulator();
+#pragma unroll
+          for (int i = 0; i < COLS / 32; ++i)
+            tmem_ld32(acc + 32 * i, z[i]);
+          release();
+        } else {
+#pragma unroll
+          for (int i = 0; i < COLS / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[i][j] = 0.0f;
+        }
+        // what rounding left of dz at the label, times the token's row of h: two columns a
+        // lane, summed over the tokens of a word, then through the slab to the word's own
+        // lane.  7 us of a step of 128 tokens (887) on a 128256 x 4096 head, below the noise
+        // of one of 4096 (12.7 ms), 15 % where thousands of tokens all have one label
+        static_assert(EPI != EPI_OUT || COLS == 64, "two columns a lane");
+        const T *h = static_cast<const T *>(a.tok.rows) + n0 + 2 * lane;
+        while (own < own_end) {
+          const int n = min(32, own_end - own);
+          float2 v = make_float2(0.0f, 0.0f);
+          auto row_of = [&](int i) -> uint32_t {
+            const long long token = __shfl_sync(~0u, own_token, i & 31);
+            if (i >= n || 2 * lane >= cols) return 0;
+            return *reinterpret_cast<const uint32_t *>(h + token * a.N);
+          };
+          uint32_t x[2] = {row_of(0), row_of(1)};  // two rows in flight
+          for (int i = 0; i < n; ++i) {
+            const int label = __shfl_sync(~0u, own_label, i);
+            const float left = __shfl_sync(~0u, own_left, i);
+            const float2 r = unpack2<T>(x[0]);
+            x[0] = x[1], x[1] = row_of(i + 2);
+            v.x = fmaf(left, r.x, v.x), v.y = fmaf(left, r.y, v.y);
+            if (i + 1 < n && __shfl_sync(~0u, own_label, i + 1) == label) continue;
+            float2 *through = reinterpret_cast<float2 *>(next_slab());
+            through[lane] = v;
+            __syncwarp();
+            if (lane == label - word0) {
+#pragma unroll
+              for (int j = 0; j < 64; j += 4) {
+                const float4 of = *reinterpret_cast<const float4 *>(through + j / 2);
+                float *o = z[j / 32] + j % 32;
+                o[0] += of.x, o[1] += of.y, o[2] += of.z, o[3] += of.w;
+              }
+            }
+            v = make_float2(0.0f, 0.0f);
+          }
+          own += n;
+          if (own + lane < own_end) {
+            own_token = a.tok.by.token[own + lane], own_label = a.tok.by.label[own + lane];
+            own_left = a.label_left[own_token];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < COLS; c += 64) {
+          if (c >= cols) break;
           unsigned char *sl = next_slab();
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            float v[32];
-            if (sums) {
-              tmem_ld32(acc + c + 32 * q, v);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-            }
+            float(&v)[32] = z[c / 32 + q];
             if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] *= scale;
@@ -739,7 +813,6 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
             store_commit();
           }
         }
-        if (sums) release();
       }
     }
     if (EPI != EPI_STATS && lane == 0) store_wait();
@@ -796,16 +869,38 @@ __global__ void __launch_bounds__(512)
   loss[t] = l;
 }
 
-// Where each counted token goes (-1: ignored), how many there are, max |g|.
+// What counting the tokens leaves in a workspace.
+struct Count {
+  int *place;          // where each counted token goes (-1: ignored)
+  int *count;          // how many there are
+  uint32_t *grad_max;  // bits of max |g|
+  ByLabel by;
+  int *other_token, *other_label;  // of the sort's alternate passes
+  int vocab;
+};
+__device__ __forceinline__ int label_key(long long label, int vocab) {
+  return label >= 0 && label < vocab ? (int)label : vocab;
+}
+
+// Counts the tokens, one block for all of them, and sorts the counted ones by label where
+// that is wanted: digits of 8 bits from the lowest on, each pass stable, 4096 tokens at a
+// time (a warp's 128 in four steps, ranked among the warp's by __match_any_sync).
 __global__ void __launch_bounds__(1024)
     vocab_count_kernel(const long long *__restrict__ labels, long long ignore,
-                       const float *__restrict__ grad, int T, int *__restrict__ place,
-                       int *__restrict__ count, uint32_t *__restrict__ grad_max) {
+                       const float *__restrict__ grad, int T, const Count c) {
   __shared__ int sums[32];
   __shared__ uint32_t tops[32];
+  __shared__ int digits[4][256];  // how often a digit occurs, then where its tokens go
+  __shared__ int by_warp[32][256];
   let_next_start();
   wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool sort = c.by.first != nullptr;
+  const int passes = sort ? (32 - __clz(c.vocab) + 7) / 8 : 0;
+  int *label = passes & 1 ? c.other_label : c.by.label;  // of the next pass
+  int *token = passes & 1 ? c.other_token : c.by.token;
+  for (int i = threadIdx.x; i < 4 * 256; i += 1024) digits[i >> 8][i & 255] = 0;
+  __syncthreads();
   int before = 0;
   uint32_t top = 0;
   for (int t0 = 0; t0 < T; t0 += 1024) {
@@ -824,7 +919,12 @@ __global__ void __launch_bounds__(1024)
     const int warps_before = __shfl_sync(~0u, v, warp) - __popc(mask);
     const int mine = before + warps_before + __popc(mask & ((1u << lane) - 1));
     before += __shfl_sync(~0u, v, 31);
-    if (t < T) place[t] = in ? mine : -1;
+    if (t < T) c.place[t] = in ? mine : -1;
+    if (sort && in) {
+      const int key = label_key(labels[t], c.vocab);
+      label[mine] = key, token[mine] = mine;
+      for (int p = 0; p < passes; ++p) atomicAdd(&digits[p][(key >> (8 * p)) & 255], 1);
+    }
     __syncthreads();
   }
 #pragma unroll
@@ -833,9 +933,74 @@ __global__ void __launch_bounds__(1024)
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 32; ++w) top = max(top, tops[w]);
-    *count = before;
-    if (grad_max) *grad_max = top;
+    *c.count = before;
+    if (c.grad_max) *c.grad_max = top;
   }
+  for (int p = 0; p < passes; ++p) {
+    int *to_label = label == c.by.label ? c.other_label : c.by.label;
+    int *to_token = token == c.by.token ? c.other_token : c.by.token;
+    if (warp == 0) {  // counts to places
+      int v[8], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = sum, sum += digits[p][8 * lane + k];
+      int all = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(~0u, all, o);
+        if (lane >= o) all += u;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) digits[p][8 * lane + k] = all - sum + v[k];
+    }
+    for (int i0 = 0; i0 < before; i0 += 4096) {
+      for (int i = threadIdx.x; i < 32 * 256; i += 1024) by_warp[i >> 8][i & 255] = 0;
+      __syncthreads();
+      int key[4], tok[4], rank[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + warp * 128 + u * 32 + lane;
+        const bool on = i < before;
+        key[u] = on ? label[i] : 0, tok[u] = on ? token[i] : 0;
+        const int d = (key[u] >> (8 * p)) & 255;
+        const uint32_t same = __match_any_sync(~0u, on ? d : 256);
+        const int seen = on ? by_warp[warp][d] : 0;
+        rank[u] = seen + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (on && (same >> lane) == 1) by_warp[warp][d] = seen + __popc(same);
+        __syncwarp();
+      }
+      __syncthreads();
+      if (threadIdx.x < 256) {
+        int at = digits[p][threadIdx.x];
+        for (int w = 0; w < 32; ++w) {
+          const int n = by_warp[w][threadIdx.x];
+          by_warp[w][threadIdx.x] = at;
+          at += n;
+        }
+        digits[p][threadIdx.x] = at;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + warp * 128 + u * 32 + lane < before) {
+          const int at = by_warp[warp][(key[u] >> (8 * p)) & 255] + rank[u];
+          to_label[at] = key[u], to_token[at] = tok[u];
+        }
+      __syncthreads();
+    }
+    label = to_label, token = to_token;
+  }
+}
+
+// first[g] of the groups after the one of the label before (-1: none) up to this one's, and
+// after the last label to the end: what the token of rank `rank` among the sorted sets.
+__device__ __forceinline__ void set_first(const ByLabel &by, int rank, int total, int before,
+                                          int label) {
+  const int from = before < 0 ? 0 : before / VL_GROUP + 1;
+  for (int g = from + threadIdx.x; g <= label / VL_GROUP; g += blockDim.x) by.first[g] = rank;
+  if (rank == total - 1)
+    for (int g = label / VL_GROUP + 1 + threadIdx.x; g <= by.groups; g += blockDim.x)
+      by.first[g] = total;
 }
 
 // The counted tokens' rows, labels, lse and g, packed; up to 63 zero rows behind them
@@ -843,46 +1008,60 @@ __global__ void __launch_bounds__(1024)
 // vocab_count_kernel's results are written here.
 template <class T, bool SELF>
 __global__ void __launch_bounds__(128)
-    vocab_gather_kernel(const T *__restrict__ h, long long ldh, int D, int tokens, int *place,
-                        int *count, uint32_t *grad_max, const long long *__restrict__ labels,
-                        long long ignore, const float *__restrict__ lse,
-                        const float *__restrict__ grad, T *__restrict__ out,
-                        long long *__restrict__ out_labels, float *__restrict__ out_lse,
-                        float *__restrict__ out_grad) {
-  __shared__ int sums[4][2];
+    vocab_gather_kernel(const T *__restrict__ h, long long ldh, int D, int tokens, const Count c,
+                        const long long *__restrict__ labels, long long ignore,
+                        const float *__restrict__ lse, const float *__restrict__ grad,
+                        T *__restrict__ out, long long *__restrict__ out_labels,
+                        float *__restrict__ out_lse, float *__restrict__ out_grad) {
+  __shared__ int sums[4][4];
   __shared__ uint32_t tops[4];
   let_next_start();
   const int t = blockIdx.x;
+  const bool sort = c.by.first != nullptr;
   int p, total;
   if (SELF) {
-    int before = 0, all = 0;
+    int before = 0, all = 0, rank = 0, last = -1;  // last: the label before in the order
     uint32_t top = 0;
+    const int own = label_key(labels[t], c.vocab);
     for (int i = threadIdx.x; i < tokens; i += 128) {
-      const bool in = labels[i] != ignore;
+      const long long label = labels[i];
+      const bool in = label != ignore;
       all += in;
       before += in && i < t;
+      const int key = label_key(label, c.vocab);
+      if (in && (key < own || (key == own && i < t))) ++rank, last = max(last, key);
       if (in && grad) top = max(top, __float_as_uint(fabsf(grad[i])));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       all += __shfl_xor_sync(~0u, all, o);
       before += __shfl_xor_sync(~0u, before, o);
+      rank += __shfl_xor_sync(~0u, rank, o);
+      last = max(last, __shfl_xor_sync(~0u, last, o));
       top = max(top, __shfl_xor_sync(~0u, top, o));
     }
     const int w = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) sums[w][0] = before, sums[w][1] = all, tops[w] = top;
+    if ((threadIdx.x & 31) == 0)
+      sums[w][0] = before, sums[w][1] = all, sums[w][2] = rank, sums[w][3] = last, tops[w] = top;
     __syncthreads();
     before = sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0];
     total = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
+    rank = sums[0][2] + sums[1][2] + sums[2][2] + sums[3][2];
+    last = max(max(sums[0][3], sums[1][3]), max(sums[2][3], sums[3][3]));
     p = labels[t] != ignore ? before : -1;
     if (threadIdx.x == 0) {
-      place[t] = p;
-      if (t == 0) *count = total, *grad_max = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+      c.place[t] = p;
+      if (t == 0)
+        *c.count = total, *c.grad_max = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+      if (sort && p >= 0) c.by.token[rank] = p, c.by.label[rank] = own;
     }
+    if (sort && p >= 0) set_first(c.by, rank, total, last, own);
   } else {
     wait_for_previous();
-    p = place[t];
-    total = *count;
+    p = c.place[t];
+    total = *c.count;
+    if (sort && t < total)
+      set_first(c.by, t, total, t ? c.by.label[t - 1] : -1, c.by.label[t]);
   }
   if (p >= 0) {
     const uint4 *in = reinterpret_cast<const uint4 *>(h + t * ldh);
@@ -1029,9 +1208,12 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // The counted tokens' place in a workspace.
 struct CountedSpace {
-  size_t place, count, gmax, labels, lse, grad, left, rows, end;
+  size_t place, count, gmax, labels, lse, grad, left, rows;
+  size_t by_token, by_label, other_token, other_label, first;  // with `words`: sorted
+  size_t end;
 };
-CountedSpace counted_space(int64_t T, int64_t D, bool grad) {
+int groups_of(int64_t words) { return (int)((words + VL_N - 1) / VL_N * (VL_N / VL_GROUP)); }
+CountedSpace counted_space(int64_t T, int64_t D, bool grad, int64_t words) {
   CountedSpace c{};
   size_t off = 0;
   auto take = [&](size_t n) {
@@ -1043,16 +1225,23 @@ CountedSpace counted_space(int64_t T, int64_t D, bool grad) {
   c.lse = take(grad ? T * 4 : 0), c.grad = take(grad ? T * 4 : 0);
   c.left = take(grad ? T * 4 : 0);
   c.rows = take((size_t)T * D * 2);
+  c.by_token = take(words ? T * 4 : 0), c.by_label = take(words ? T * 4 : 0);
+  c.other_token = take(words ? T * 4 : 0), c.other_label = take(words ? T * 4 : 0);
+  c.first = take(words ? (groups_of(words) + 1) * 4ll : 0);
   c.end = off;
   return c;
 }
 template <class T>
 int gather_counted(const void *h, const Shape &z, const long long *labels, long long ignore,
-                   const float *lse, const float *grad, char *ws, const CountedSpace &c,
-                   Counted *tok, cudaStream_t s) {
-  int *place = reinterpret_cast<int *>(ws + c.place);
-  int *count = reinterpret_cast<int *>(ws + c.count);
-  auto *gmax = reinterpret_cast<uint32_t *>(ws + c.gmax);
+                   const float *lse, const float *grad, bool sorted, char *ws,
+                   const CountedSpace &c, Counted *tok, cudaStream_t s) {
+  auto ints = [&](size_t at) { return reinterpret_cast<int *>(ws + at); };
+  Count n{ints(c.place), ints(c.count), reinterpret_cast<uint32_t *>(ws + c.gmax)};
+  n.vocab = z.V;
+  if (sorted) {
+    n.by = {ints(c.by_token), ints(c.by_label), ints(c.first), groups_of(z.V)};
+    n.other_token = ints(c.other_token), n.other_label = ints(c.other_label);
+  }
   auto *lab = reinterpret_cast<long long *>(ws + c.labels);
   float *l = reinterpret_cast<float *>(ws + c.lse), *g = reinterpret_cast<float *>(ws + c.grad);
   // the first of its chain waits for all before it.  Up to 1024 tokens every block of
@@ -1061,19 +1250,19 @@ int gather_counted(const void *h, const Shape &z, const long long *labels, long 
   const T *from = static_cast<const T *>(h);
   if (z.T <= 1024) {
     if (int rc = launch_chained(vocab_gather_kernel<T, true>, dim3(z.T), dim3(128), 0, 1, false, s,
-                                from, z.ldh, z.D, z.T, place, count, gmax, labels, ignore, lse,
-                                grad, rows, lab, l, g))
+                                from, z.ldh, z.D, z.T, n, labels, ignore, lse, grad, rows, lab, l,
+                                g))
       return rc;
   } else {
     if (int rc = launch_chained(vocab_count_kernel, dim3(1), dim3(1024), 0, 1, false, s, labels,
-                                ignore, grad, z.T, place, count, gmax))
+                                ignore, grad, z.T, n))
       return rc;
     if (int rc = launch_chained(vocab_gather_kernel<T, false>, dim3(z.T), dim3(128), 0, 1, true, s,
-                                from, z.ldh, z.D, z.T, place, count, gmax, labels, ignore, lse,
-                                grad, rows, lab, l, g))
+                                from, z.ldh, z.D, z.T, n, labels, ignore, lse, grad, rows, lab, l,
+                                g))
       return rc;
   }
-  *tok = Counted{count, lab, l, g, gmax};
+  *tok = Counted{n.count, lab, l, g, n.grad_max, rows, n.by};
   return B2F_OK;
 }
 
@@ -1123,7 +1312,7 @@ Plan grad_plan(int64_t T, int64_t V, int64_t D, bool need_h, int sms) {
     const int64_t cost = ((tiles * n + slots - 1) / slots) * (per + 6);
     if (!best || cost < best) best = cost, p.splits = (int)n;
   }
-  p.c = counted_space(T, D, true);
+  p.c = counted_space(T, D, true, dz_in_two(T) ? 0 : V);
   size_t off = p.c.end;
   p.dz = off, off += round256((size_t)rows * p.piece * 2);
   p.partial = off;
@@ -1162,8 +1351,9 @@ int forward(const void *h, const void *w, const Shape &z, const long long *label
   const int *place = nullptr;
   long long ldh = z.ldh;
   if (forward_gathers(z.T)) {
-    const CountedSpace c = counted_space(z.T, z.D, false);
-    if (int rc = gather_counted<T>(h, z, labels, ignore, nullptr, nullptr, ws + off, c, &a.tok, s))
+    const CountedSpace c = counted_space(z.T, z.D, false, 0);
+    if (int rc = gather_counted<T>(h, z, labels, ignore, nullptr, nullptr, false, ws + off, c,
+                                   &a.tok, s))
       return rc;
     h = ws + off + c.rows;
     ldh = z.D;
@@ -1187,9 +1377,10 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
   float *partial = reinterpret_cast<float *>(ws + p.partial);
   float *left = reinterpret_cast<float *>(ws + p.c.left);
   Counted tok;
-  if (int rc = gather_counted<T>(h, z, labels, ignore, lse, grad, ws, p.c, &tok, s)) return rc;
-  const int group = blocks_per_tile(z.T);
   const int low = dz_in_two(z.T) ? z.T : 0, rows = (int)dz_rows(z.T);
+  if (int rc = gather_counted<T>(h, z, labels, ignore, lse, grad, dw && !low, ws, p.c, &tok, s))
+    return rc;
+  const int group = blocks_per_tile(z.T);
   CUtensorMap h_k, h_n, w_k, w_n, dz_k, dz_m, dz_out, sums, dw_out;
   if (int rc = encode_map<T>(&h_k, hc, z.T, z.D, z.D, VL_M)) return rc;
   if (int rc = encode_map<T>(&w_k, w, z.V, z.D, z.ldw, VL_N / group)) return rc;
@@ -1231,7 +1422,8 @@ int backward(const void *h, const void *w, const Shape &z, const long long *labe
       b.M = words, b.N = z.D, b.K = rows, b.splits = 1, b.low = low;
       b.m_first = v0;
       b.tok = tok, b.tokens_in_k = 1;
-      if (int rc = launch_gemm<T, EPI_OUT, true, true>(dz_m, h_n, dw_out, b, 2, true, dev, sms, s))
+      b.label_left = left;
+      if (int rc = launch_tiles<T, EPI_OUT, true, true, 2>(dz_m, h_n, dw_out, b, true, dev, sms, s))
         return rc;
     }
   }
@@ -1256,7 +1448,7 @@ size_t b2f_vocab_loss_workspace(int64_t T, int64_t V, int64_t D) {
   int dev = 0, sms = 0;
   if (T < 1 || V < 1 || D < 1 || current_device(&dev, &sms)) return 0;
   return round256((size_t)T * 4) + round256((size_t)forward_slots(T, V, sms) * T * 8) +
-         (forward_gathers(T) ? counted_space(T, D, false).end : 0);
+         (forward_gathers(T) ? counted_space(T, D, false, 0).end : 0);
 }
 
 int b2f_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int dtype,

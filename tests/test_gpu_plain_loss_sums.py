@@ -1,0 +1,106 @@
+"""What the sums of the vocabulary loss's gradients keep (csrc/vocab_loss.cu), against
+binary64."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from _plain import half_step, loss64, loss_grad64
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+def _inputs(t, v, d, dtype, ignored=0.2, seed=0, lean=12.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randn((v, d), generator=g, device="cuda") / d ** 0.5).to(dtype)
+    labels = torch.randint(0, v, (t,), generator=g, device="cuda")
+    h = torch.randn((t, d), generator=g, device="cuda")
+    h = (h + lean * torch.rand((t, 1), generator=g, device="cuda") * w[labels]).to(dtype)
+    off = torch.rand((t,), generator=g, device="cuda") < ignored
+    labels = torch.where(off, torch.full_like(labels, -100), labels)
+    grad = torch.randn((t,), generator=g, device="cuda") / t
+    return h, w, labels, grad
+
+
+def _weight_gradient_is_exact_at_labels(h, w, labels, grad, dw):
+    """dz is rounded by up to half a step at every word but the label, whose remainder is
+    added in binary32: there only half a step squared is lost (2^-24 of it), and each token
+    of a word costs its row of dW one rounding more.  A p is off by twice a logit's error e
+    ((d / 16 + 2) accumulations of 2^-22 max|z|, and lse's 16 steps) and by 2^-20 for the
+    exponential and its argument; a sum by a step of 2^-22 of its terms for every 16 tokens;
+    the output by half a step.  Below 2^-126 nothing keeps its relative precision, in fp16
+    below 2^-38 max|g| (dz under its scale) and 2^-25 (the output)."""
+
+    t, d = h.shape
+    dz = loss_grad64(h, w, labels, -100, grad)
+    _, lse, z = loss64(h, w, labels, -100)
+    e = (d / 16 + 2) * 2.0 ** -22 * float(z.abs().max()) + 16 * 2.0 ** -23 * lse.abs().clamp(min=1.0)
+    counted = labels != -100
+    g = torch.where(counted, grad.double().abs(), 0.0)[:, None]
+    step = half_step(h.dtype)
+    lost = torch.full_like(dz, 1.01 * step)
+    lost[torch.arange(t), labels.clamp(min=0)] = 2.0 ** -24
+    size = dz.abs() * (lost + 2.0 ** -20) + 2 * e[:, None] * torch.exp(z - lse[:, None]) * g
+    size += 2.0 ** -126
+    if h.dtype == FP:
+        size += 2.0 ** -38 * float(g.max()) * counted[:, None]
+    hc = torch.where(counted[:, None], h.double(), 0.0)
+    want, total = dz.T @ hc, dz.abs().T @ hc.abs()
+    each = torch.bincount(labels[counted], minlength=w.shape[0])[:, None]
+    tol = size.T @ hc.abs() + ((t / 16 + 16) * 2.0 ** -22 + (each + 1) * 2.0 ** -24) * total
+    tol = tol + 1.01 * step * want.abs() + 2.0 ** -126 + (2.0 ** -25 if h.dtype == FP else 0.0)
+    diff = (dw.double() - want).abs()
+    assert bool((diff <= tol).all()), float((diff / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,v,d", [(65, 300, 64), (130, 2000, 200), (300, 40, 72), (1100, 700, 72),
+                                   (1024, 70000, 64), (1025, 255, 8), (9000, 70001, 24)])
+def test_weight_gradient_keeps_the_labels_dz(dtype, t, v, d):
+    from easyfhe import plain
+
+    h, w, labels, grad = _inputs(t, v, d, dtype)
+    _, lse = plain.vocab_loss(h, w, labels)
+    dh, dw = plain.vocab_loss_grad(h, w, labels, lse, grad)
+    _weight_gradient_is_exact_at_labels(h, w, labels, grad, dw)
+    again = plain.vocab_loss_grad(h, w, labels, lse, grad, need_hidden=False)[1]
+    assert torch.equal(again, dw)
+
+
+@pytest.mark.parametrize("t", [70, 1000, 3000])
+@pytest.mark.parametrize("which", ["one", "ends", "few", "last counted"])
+def test_labels_that_many_tokens_share(t, which):
+    from easyfhe import plain
+
+    v = 777
+    h, w, labels, grad = _inputs(t, v, 200, BF, lean=0.0)
+    at = torch.arange(t, device="cuda")
+    labels = {"one": torch.full_like(labels, 5), "ends": torch.where(at % 3 == 0, 0, v - 1),
+              "few": 31 + at % 4,
+              "last counted": torch.where(at == t - 1, 256, -100)}[which]
+    _, lse = plain.vocab_loss(h, w, labels)
+    dh, dw = plain.vocab_loss_grad(h, w, labels, lse, grad)
+    _weight_gradient_is_exact_at_labels(h, w, labels, grad, dw)
+
+
+def test_labels_outside_the_vocabulary_among_many():
+    """A label that is no word makes every row of dW NaN (its token's dz is), and leaves the
+    other tokens' rows of dh what they are without it."""
+    from easyfhe import plain
+
+    for t in (100, 2000):
+        h, w, labels, grad = _inputs(t, 300, 64, BF)
+        labels[7] = -100
+        _, lse = plain.vocab_loss(h, w, labels)
+        clean, dw = plain.vocab_loss_grad(h, w, labels, lse, grad)
+        assert torch.isfinite(dw).all()
+        for bad in (300, -3, 2 ** 40):
+            labels[7] = bad
+            _, lse = plain.vocab_loss(h, w, labels)
+            dh, dw = plain.vocab_loss_grad(h, w, labels, lse, grad)
+            assert torch.isnan(dw).all() and torch.isnan(dh[7]).all()
+            keep = torch.arange(t, device="cuda") != 7
+            assert torch.equal(dh[keep], clean[keep])
