@@ -274,11 +274,14 @@ __device__ __forceinline__ void q4_values(const Q4Args &a, int tile0, int tiles,
 
 // x as digits: digits [tile][8 NT][4 lanes][4 words] of 4 bytes (a word's columns 0, 2,
 // 1, 3: the order of its nibbles), factor [tile][8 NT] = 256^plane
-// 2^-sh.  Columns past the last one are zero.  An infinite or NaN x makes plane 0
-// alone, with digits +-1 at infinities and an infinite (NaN) factor.
+// 2^-sh.  Columns past the last one are zero.  A NaN among x makes every sum of its row
+// and tile NaN by plane 0's factor.  Infinities are no digits: their sum must not cancel
+// before it is infinite.  They leave +-1 in plane 0 under a factor of -0, which marks them
+// for q4_infinite.  Returns whether this thread met infinities.
 template <int NT>
-__device__ __forceinline__ void q4_digits(const Q4Args &a, int tile0, int tiles,
+__device__ __forceinline__ bool q4_digits(const Q4Args &a, int tile0, int tiles,
                                           unsigned char *digits, float *factor) {
+  bool infinite = false;
   const int idle = 2 * NT - a.rows;  // rows past the last one
   for (int i = threadIdx.x; i < tiles * idle * 16; i += blockDim.x) {
     const int kt = (i >> 4) / idle, c = 4 * a.rows + (((i >> 4) - kt * idle) << 2);
@@ -327,10 +330,62 @@ __device__ __forceinline__ void q4_digits(const Q4Args &a, int tile0, int tiles,
     o[48] = __byte_perm(a23, b23, 0x7632);
     if (q < 4) {
       float x = __uint_as_float((uint32_t)max(127 + 8 * q - sh, 1) << 23);
-      if (e == 255) x = q ? 0.0f : __uint_as_float(top);  // infinity or NaN
+      if (e == 255) {
+        x = q ? 0.0f : top == 0x7f800000u ? -0.0f : __uint_as_float(top);
+        infinite |= top == 0x7f800000u;
+      }
       factor[kt * 8 * NT + row * 4 + q] = x;
     }
   });
+  return infinite;
+}
+
+// What the infinities of row b of x among a block's tiles make of the sums of weight rows g
+// and g + 8 of row block rb: in each tile and group an infinity of the sign that all its
+// products have, or NaN where they differ or one has a zero weight; 0 without infinities.
+template <int NT, bool ZERO, bool G32, bool SB>
+__device__ __noinline__ float2 q4_infinite(const Q4Args &a, int rb, int b, int tile0, int tiles,
+                                           const unsigned char *digits, const float *factor) {
+  constexpr int REC = q4_record(G32, ZERO), SUB = G32 ? 2 : 1;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float2 sum = make_float2(0.0f, 0.0f);
+  for (int kt = 0; kt < tiles; ++kt) {
+    const int col = kt * 8 * NT + 4 * b;
+    if (__float_as_uint(factor[col]) != 0x80000000u) continue;
+    const unsigned char *p = a.packed + ((long long)rb * a.tiles_k + tile0 + kt) * REC;
+    const uint4 c = reinterpret_cast<const uint4 *>(p)[lane];
+    const uint4 d = reinterpret_cast<const uint4 *>(digits)[col * 4 + t];
+    const uint32_t code[4] = {c.x, c.y, c.z, c.w}, mark[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+      int z0 = 8, z1 = 8;
+      if (ZERO) {
+        const uint16_t z = reinterpret_cast<const uint16_t *>(p + q4_zeros_at(G32))[8 * u + g];
+        z0 = z & 255, z1 = z >> 8;
+      }
+      uint32_t seen = 0;  // 1: positive products, 2: negative, 4: of nothing; << 3 for row g + 8
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        if (G32 && u != m / 2) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int sign = (int)(signed char)(mark[m] >> (8 * k));
+          const int p0 = sign * ((int)((code[m] >> (8 * k)) & 15u) - z0);
+          const int p1 = sign * ((int)((code[m] >> (8 * k + 4)) & 15u) - z1);
+          if (sign)
+            seen |= (p0 > 0 ? 1u : p0 < 0 ? 2u : 4u) | (p1 > 0 ? 8u : p1 < 0 ? 16u : 32u);
+        }
+      }
+      seen |= __shfl_xor_sync(~0u, seen, 1);
+      seen |= __shfl_xor_sync(~0u, seen, 2);
+      if (!seen) continue;
+      auto value = [](uint32_t v) { return v == 1 ? INFINITY : v == 2 ? -INFINITY : NAN; };
+      const float2 s = scale_pair<SB>(reinterpret_cast<const uint32_t *>(p + 512)[8 * u + g]);
+      sum.x += s.x * value(seen & 7u);
+      sum.y += s.y * value(seen >> 3);
+    }
+  }
+  return sum;
 }
 
 // first [tile][SUB][4 NT]: the accumulators' first values of two columns, twice (-8 sum
@@ -390,6 +445,61 @@ constexpr int q4_max_warps(Q4Rows how) { return how == Q4_DIGITS ? 8 : 16; }
 constexpr int q4_digit_bytes(int nt) { return 512 * nt; }
 constexpr int q4_tile_bytes(bool digits, bool g32, int nt, int cols) {
   return digits ? q4_digit_bytes(nt) + ((g32 ? 2 : 1) * 64 + 32) * nt : cols * 128;
+}
+
+// Infinities join y when all else is there, a row block to a warp and a cluster's blocks one
+// after the other.  Within the loop over the records, on its registers, they cost four rows
+// of 128256 x 4096 14 us of 84 without one infinity among them.  A call, and ids read again,
+// leave the loop its registers: one to four rows take as long as without (zero points: 1 %).
+template <int NT, bool ZERO, bool G32, bool SB>
+__device__ __forceinline__ void q4_join_infinite(const Q4Args &a) {
+  extern __shared__ __align__(16) unsigned char q4_smem[];
+  const unsigned char *xs = q4_smem + 16;
+  const float *factor =
+      reinterpret_cast<const float *>(xs + (size_t)a.block_tiles *
+                                               (q4_digit_bytes(NT) + (G32 ? 2 : 1) * 64 * NT));
+  const int cs = a.cluster;
+  if (cs == 1) {
+    __syncthreads();
+    if (!*reinterpret_cast<volatile int *>(q4_smem)) return;
+  }
+  uint32_t tid, block_id;
+  asm volatile("mov.u32 %0, %%tid.x;\n" : "=r"(tid));
+  asm volatile("mov.u32 %0, %%ctaid.x;\n" : "=r"(block_id));
+  const int warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31, warps = blockDim.x >> 5;
+  const int rank = cs == 1 ? 0 : (int)cluster_rank();
+  const int row_blocks = (a.N + Q4_ROWS - 1) / Q4_ROWS, wr = a.warps_r;
+  const int stride = gridDim.x / cs * wr, tile0 = rank * a.block_tiles;
+  const int tiles = max(0, min(a.block_tiles, a.tiles_k - tile0));
+  auto add = [](auto *y, float v) { *y = (std::remove_pointer_t<decltype(y)>)((float)*y + v); };
+#pragma unroll 1
+  for (int turn = 0; turn < cs; ++turn) {
+    if (turn == rank && *reinterpret_cast<volatile int *>(q4_smem)) {
+#pragma unroll 1
+      for (int i = warp, b0 = (int)block_id / cs * wr;; i += warps) {
+        while (i >= wr && b0 < row_blocks) i -= wr, b0 += stride;
+        if (b0 >= row_blocks) break;
+        if (b0 + i >= row_blocks) continue;
+#pragma unroll 1
+        for (int b = 0; b < a.rows; ++b) {
+          const float2 v = q4_infinite<NT, ZERO, G32, SB>(a, b0 + i, b, tile0, tiles, xs, factor);
+          const long long n = (long long)(b0 + i) * Q4_ROWS + (lane >> 2), at = b * a.ldy + n;
+#pragma unroll 1
+          for (int r = 0; r < 2; ++r) {
+            const float w = r ? v.y : v.x;
+            if ((lane & 3) != 0 || w == 0.0f || n + 8 * r >= a.N) continue;
+            if (a.out_f32 || a.dtype == B2F_F32)
+              add(static_cast<float *>(a.y) + at + 8 * r, w);
+            else if (a.dtype == B2F_F16)
+              add(static_cast<__half *>(a.y) + at + 8 * r, w);
+            else
+              add(static_cast<__nv_bfloat16 *>(a.y) + at + 8 * r, w);
+          }
+        }
+      }
+    }
+    if (cs > 1) meet(cs);
+  }
 }
 
 // In round i cluster c takes the warps_r row blocks from (c + i clusters) warps_r on;
@@ -452,8 +562,8 @@ __global__ void __launch_bounds__(32 * q4_max_warps(HOW), HOW == Q4_DIGITS ? 2 :
 
   if (threadIdx.x == 0) *reinterpret_cast<uint4 *>(q4_smem) = make_uint4(0, 0, 0, 0);
   if constexpr (INT) {
-    q4_digits<NT>(a, tile0, tiles, xs, factor);
-    __syncthreads();
+    const int infinite = __syncthreads_or(q4_digits<NT>(a, tile0, tiles, xs, factor));
+    if (threadIdx.x == 0) reinterpret_cast<uint4 *>(q4_smem)->x = infinite;
     q4_first<NT, ZERO, G32>(tiles, xs, first);
   } else {
     q4_values<SPLIT>(a, tile0, tiles, xs);
@@ -629,7 +739,7 @@ __global__ void __launch_bounds__(32 * q4_max_warps(HOW), HOW == Q4_DIGITS ? 2 :
       float v = 0.0f;
 #pragma unroll 4
       for (int u = 0; u < wk; ++u, s += SUMS) {
-        if (INT)  // small digits first; a row that is not finite has one plane alone
+        if (INT)  // small digits first; what is not finite is in plane 0 alone
           v += s[4 * b + 3] + (s[4 * b + 2] + (s[4 * b + 1] + s[4 * b]));
         else if (SPLIT)
           v += s[3 * b] + (s[3 * b + 2] + s[3 * b + 1]);
@@ -655,6 +765,7 @@ __global__ void __launch_bounds__(32 * q4_max_warps(HOW), HOW == Q4_DIGITS ? 2 :
     buf ^= 1;
   }
   if (cs > 1) meet(cs);  // no block leaves while its sums are read
+  if constexpr (INT) q4_join_infinite<NT, ZERO, G32, SB>(a);
 }
 
 // codes [N][K] (one byte each), scales and zero points [N][groups] -> records.
