@@ -25,8 +25,9 @@
 // with more than 128 tokens) two blocks of a cluster tiles of 256 x 256
 // (cta_group::2), each loading half of both operands: 32 KB a K step instead of 48
 // for as much of the product.  Outputs leave through shared memory as TMA
-// stores.  Every wait is bounded: a wait that runs out ends the block and is counted
-// (b2f_vocab_loss_wait_errors).
+// stores.  Every wait is bounded: one that runs out is counted (b2f_vocab_loss_wait_errors),
+// the block waits (bounded again) for its loads and products in flight, and all tiles that
+// it still owes are NaN, which whatever is computed from them hands on.
 //
 // dz is rounded to the operand type before its two products (once from 65 tokens
 // on: relative to each dz at most half a step of the type, the size of the rounding of
@@ -84,6 +85,7 @@ static_assert(Block<1>::smem <= 227 * 1024 && Block<2>::smem <= 227 * 1024,
 // Both passes over the logits cut them alike, for the errors of z and lse to cancel in dz.
 constexpr int VL_CHUNK = 8;
 constexpr int VL_WAIT_LIMIT = 1 << 23;  // polls (each may suspend the thread for a while)
+constexpr int VL_IDLE_LIMIT = 1 << 10;  // where nothing is to come (VocabArgs::idle)
 
 __device__ int g_vocab_wait_errors;
 
@@ -134,6 +136,7 @@ struct VocabArgs {
   float *label_logit; // [M]
   float *label_left;  // [M] what rounding left of dz at the label
   int accumulate;     // dh: add to the partial sums
+  int idle;           // blocks (or pairs) from 1: this one loads nothing, its waits run out
 };
 
 // The tiles of a product, as every warp counts them off.
@@ -193,8 +196,9 @@ __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
   return done;
 }
 // bounded; false when the wait ran out here or in another warp (*lost set)
-__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *lost) {
-  for (int it = 0; it < VL_WAIT_LIMIT; ++it) {
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatile int *lost,
+                                         int limit = VL_WAIT_LIMIT) {
+  for (int it = 0; it < limit; ++it) {
     if (bar_try(bar, parity)) return true;
     if (*lost) return false;
   }
@@ -448,7 +452,8 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
   unsigned char *slabs = base + STAGES * B::stage;
   uint64_t *full = reinterpret_cast<uint64_t *>(slabs + B::warps * VL_SLAB);
   uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
-  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  uint64_t *drained = acc_empty + 2;
+  uint32_t *tmem_ptr = reinterpret_cast<uint32_t *>(drained + 1);
   volatile int *lost = reinterpret_cast<volatile int *>(tmem_ptr + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   let_next_start();
@@ -457,6 +462,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) bar_init(full + s, 1), bar_init(empty + s, 1);
     for (int s = 0; s < 2; ++s) bar_init(acc_full + s, 1), bar_init(acc_empty + s, CG * B::warps);
+    bar_init(drained, 1);
     *lost = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -487,10 +493,11 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
   const Tiles ts = tiles_of<CG>(a, M, K);
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
   const bool sums = ts.k_blocks > 0;  // no counted token: dW is zero without a product
+  const bool idle = a.idle == first + 1;
+  int it = 0;  // K steps loaded (warp 0) or multiplied (warp 1)
 
   if (warp == 0) {
-    if (lane == 0 && sums) {
-      int it = 0;
+    if (lane == 0 && sums && !idle) {
       bool ok = true;
       for (int tile = first; tile < ts.total && ok; tile += step) {
         const Tile at = tile_at<EPI>(ts, tile);
@@ -522,19 +529,14 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
           }
         }
       }
-      if (!ok && rank == 0)  // let the loads in flight land before the block ends
-        for (int i = max(0, it - STAGES); i < it; ++i)
-          for (int p = 0; p < VL_WAIT_LIMIT && !bar_try(full + i % STAGES, (i / STAGES) & 1);
-               ++p) {
-          }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0 && sums) {
+    if (lane == 0 && rank == 0 && sums && !idle) {
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)AMN << 15) |
                                  ((uint32_t)BMN << 16) | ((uint32_t)(VL_N >> 3) << 17) |
                                  ((uint32_t)(TILE_M >> 4) << 24);
-      int it = 0, n = 0;
+      int n = 0;
       bool ok = true;
       for (int tile = first; tile < ts.total && ok; tile += step) {
         const int split = tile_at<EPI>(ts, tile).split;
@@ -571,6 +573,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
       scale = dz_scale(a.tok.grad_max);
     if (EPI != EPI_DZ) scale = 1.0f / scale;
     float run_max = -INFINITY, run_rest = -1.0f;  // stats of one row over a block's tiles
+    bool ok = true;  // no wait of this warp ran out; none of its tiles is there after one did
     for (int tile = first; tile < ts.total; tile += step) {
       const Tile where = tile_at<EPI>(ts, tile);
       const int mt = where.m, nt = where.n, split = where.split;
@@ -580,7 +583,8 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
         return tmem + (n & 1) * VL_N + part * COLS + ((uint32_t)(quarter * 32) << 16);
       };
       auto ready = [&]() {
-        const bool ok = __all_sync(~0u, bar_wait(acc_full + (n & 1), (n >> 1) & 1, lost));
+        ok = ok && __all_sync(~0u, bar_wait(acc_full + (n & 1), (n >> 1) & 1, lost,
+                                            idle ? VL_IDLE_LIMIT : VL_WAIT_LIMIT));
         fence_after();
         return ok;
       };
@@ -602,9 +606,8 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
       };
       if constexpr (LOGITS) {
         float z[COLS / 32][32];
-        bool ok = true;
-        for (int kc = 0; kc < ts.k_blocks && ok; kc += VL_CHUNK) {
-          if (!(ok = ready())) break;
+        for (int kc = 0; kc < ts.k_blocks; kc += VL_CHUNK) {
+          if (!ready()) break;
           const uint32_t acc = accumulator();
 #pragma unroll
           for (int i = 0; i < COLS / 32; ++i)
@@ -623,7 +626,12 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
             }
           release();
         }
-        if (!ok) break;
+        if (!ok) {
+#pragma unroll
+          for (int i = 0; i < COLS / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z[i][j] = NAN;
+        }
         const bool live = t < M;
         const long long label = live ? a.tok.labels[t] : a.ignore;
         const long long at = label - a.n_first - n0;  // the label's column here
@@ -711,12 +719,17 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
                 make_float2(mx, rest);
         }
       } else if constexpr (EPI == EPI_PARTIAL) {
-        if (!ready()) break;
+        const bool there = ready();
         const uint32_t acc = accumulator();
         for (int c = 0; c < COLS && c < cols; c += 32) {
           unsigned char *sl = next_slab();
           float v[32];
-          tmem_ld32(acc + c, v);
+          if (there) {
+            tmem_ld32(acc + c, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = NAN;
+          }
           put_floats(sl, lane, v);
           filled();
           const int r = m0 + quarter * 32;
@@ -725,7 +738,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
             store_commit();
           }
         }
-        release();
+        if (there) release();
       } else {
         // the tokens whose label is one of this warp's words, the first 32 of them in its
         // lanes: asked for before the wait
@@ -740,8 +753,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
           }
         }
         float z[COLS / 32][32];
-        if (sums) {
-          if (!ready()) break;
+        if (sums && ready()) {
           const uint32_t acc = accumulator();
 #pragma unroll
           for (int i = 0; i < COLS / 32; ++i)
@@ -751,7 +763,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
 #pragma unroll
           for (int i = 0; i < COLS / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) z[i][j] = 0.0f;
+            for (int j = 0; j < 32; ++j) z[i][j] = ok ? 0.0f : NAN;
         }
         // what rounding left of dz at the label, times the token's row of h: two columns a
         // lane, summed over the tokens of a word, then through the slab to the word's own
@@ -820,6 +832,20 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
   __syncwarp();
   fence_before();
   __syncthreads();
+  if (*lost && rank == 0) {
+    // loads in flight (all of a pair's arrive at its first block) and products end before
+    // their memory is freed
+    if (threadIdx.x == 0)
+      for (int i = max(0, it - STAGES); i < it; ++i)
+        for (int p = 0; p < VL_WAIT_LIMIT && !bar_try(full + i % STAGES, (i / STAGES) & 1); ++p) {
+        }
+    if (threadIdx.x == 32) {
+      mma_commit<CG>(drained);
+      for (int p = 0; p < VL_WAIT_LIMIT && !bar_try(drained, 0); ++p) {
+      }
+    }
+    __syncwarp();
+  }
   if (CG > 1) cluster_meet();
   fence_after();
   if (warp == 1) {
@@ -1179,9 +1205,14 @@ int encode_partial(CUtensorMap *m, const float *p, long long splits, long long r
 // bound every product and half of a 256-row tile would be empty.
 int blocks_per_tile(int64_t T) { return T > VL_M ? 2 : 1; }
 
+// b2f_vocab_loss_idle_block's product (low byte) and block from 1 (the rest); 0: none
+std::atomic<int64_t> g_idle{0};
+
 template <class T, int EPI, bool AMN, bool BMN, int CG>
-int launch_tiles(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo,
-                 const VocabArgs &a, bool chained, int dev, int sms, cudaStream_t s) {
+int launch_tiles(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, VocabArgs a,
+                 bool chained, int dev, int sms, cudaStream_t s) {
+  const int64_t idle = g_idle.load(std::memory_order_relaxed);
+  a.idle = (idle & 255) == EPI ? (int)(idle >> 8) : 0;
   auto k = vocab_gemm_kernel<T, EPI, AMN, BMN, CG>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared(k, (int)Block<CG>::smem, dev, allowed)) return rc;
@@ -1513,6 +1544,14 @@ int b2f_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int
                                 grad_weight, p, w, dev, sms, s)
              : backward<__nv_bfloat16>(hidden, weight, z, lab, ignore, lse, grad_loss,
                                        grad_hidden, grad_weight, p, w, dev, sms, s);
+}
+
+int b2f_vocab_loss_idle_block(int product, int block) {
+  using namespace b2f;
+  B2F_CHECK_ARG(product >= 0 && product <= 3 && block >= -1 && block < (1 << 20),
+                "b2f_vocab_loss_idle_block: product %d, block %d", product, block);
+  g_idle.store(((int64_t)(block + 1) << 8) | product, std::memory_order_relaxed);
+  return B2F_OK;
 }
 
 int b2f_vocab_loss_wait_errors(void) {

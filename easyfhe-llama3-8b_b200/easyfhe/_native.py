@@ -132,6 +132,7 @@ _SIGS = {
     "b2f_vocab_loss_grad": (_int, [_vp, _i64, _vp, _i64, _int, _i64, _i64, _i64, _vp, _i64, _vp,
                                    _vp, _vp, _vp, _vp, _size, _vp]),
     "b2f_vocab_loss_wait_errors": (_int, []),
+    "b2f_vocab_loss_idle_block": (_int, [_int, _int]),
 }
 
 

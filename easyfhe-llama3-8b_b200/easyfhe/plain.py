@@ -429,7 +429,8 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
     hidden [tokens, D], weight [words, D] (both f16 or both bf16, D a multiple
     of 8; rows off 16-byte boundaries cost a copy), labels int64.  A label of
     ignore_index gives 0 for both; any other label outside the vocabulary gives a
-    loss of NaN, as do logits that overflow."""
+    loss of NaN, as do logits that overflow (and sums that the device did not
+    deliver, which `wait_errors` counts)."""
 
     index, t, v, d = _loss_args("vocab_loss", hidden, weight, labels)
     if _current_device() != index:
@@ -487,3 +488,16 @@ def vocab_loss_grad(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     if rc:
         check(rc, "vocab_loss_grad")
     return dh, dw
+
+
+def wait_errors(device: str | torch.device | None = None) -> int:
+    """How many waits inside `vocab_loss` and `vocab_loss_grad` ran out on a device
+    (the current one) since the library was loaded: 0 on a healthy device.  What was
+    waited for is NaN in their results.  Waits for the device."""
+
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        count = lib.b2f_vocab_loss_wait_errors()
+    if count < 0:
+        raise RuntimeError("wait_errors: the device's counter cannot be read")
+    return count

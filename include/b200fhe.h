@@ -542,10 +542,16 @@ int b2f_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int
                         int64_t ignore, const float *lse, const float *grad_loss,
                         void *grad_hidden, void *grad_weight, void *ws, size_t ws_bytes,
                         void *stream);
-/* Waits of the two calls above that ran out (the block ended, its outputs are
- * not written) since the library loaded, on the current device; 0 on a
- * healthy run, -1 when the counter cannot be read. */
+/* Waits of the two calls above that ran out since the library loaded, on the
+ * current device; 0 on a healthy run, -1 when the counter cannot be read.  What a
+ * call owes after such a wait is NaN: the loss and lse of the tokens concerned,
+ * their rows of grad_hidden, the words' rows of grad_weight. */
 int b2f_vocab_loss_wait_errors(void);
+/* For tests of that: from the next call on, thread block `block` (or pair of
+ * blocks; -1: none) of product 0 (the loss's logits), 1 (the gradient's), 2
+ * (grad_hidden) or 3 (grad_weight) loads and multiplies nothing, so that the waits
+ * for its sums run out, after a short time. */
+int b2f_vocab_loss_idle_block(int product, int block);
 
 #ifdef __cplusplus
 }
