@@ -84,6 +84,11 @@ static_assert(Block<1>::smem <= 227 * 1024 && Block<2>::smem <= 227 * 1024,
 // of 256 halve the error again and cost 7 % (and 12 % of a step on 4096 tokens).
 // Both passes over the logits cut them alike, for the errors of z and lse to cancel in dz.
 constexpr int VL_CHUNK = 8;
+// K steps of a gradient that they add up in one go, for the same reason: up to 1024 truncations,
+// 1.2e-4 of a sum of one sign, a quarter of what rounding it to fp16 may cost.  dW of 2^20
+// tokens with positive terms, in fp16, is off by 6e-5 to 9e-5 on average, in one go by 5.8e-3
+// (in stretches of 1024 steps by up to 3.9e-4).
+constexpr int VL_LONG = 256;
 constexpr int VL_WAIT_LIMIT = 1 << 23;  // polls (each may suspend the thread for a while)
 constexpr int VL_IDLE_LIMIT = 1 << 10;  // where nothing is to come (VocabArgs::idle)
 
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
       for (int tile = first; tile < ts.total && ok; tile += step) {
         const int split = tile_at<EPI>(ts, tile).split;
         const int kb0 = split * ts.split_blocks, kb1 = min(kb0 + ts.split_blocks, ts.k_blocks);
-        const int chunk = LOGITS ? VL_CHUNK : ts.split_blocks;
+        constexpr int chunk = LOGITS ? VL_CHUNK : VL_LONG;
         for (int kc = kb0; kc < kb1 && ok; kc += chunk, ++n) {
           const int buf = n & 1, end = min(kc + chunk, kb1);
           if (n >= 2 && !(ok = bar_wait(acc_empty + buf, ((n >> 1) - 1) & 1, lost))) break;
@@ -604,15 +609,16 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         __syncwarp();
       };
-      if constexpr (LOGITS) {
-        float z[COLS / 32][32];
-        for (int kc = 0; kc < ts.k_blocks; kc += VL_CHUNK) {
+      // the tile's sums of this warp, its chunks joined; NaN where a wait ran out
+      auto collect = [&](float(&z)[COLS / 32][32], int kb0, int kb1) {
+        constexpr int chunk = LOGITS ? VL_CHUNK : VL_LONG;
+        for (int kc = kb0; kc < kb1; kc += chunk) {
           if (!ready()) break;
           const uint32_t acc = accumulator();
 #pragma unroll
           for (int i = 0; i < COLS / 32; ++i)
-            if (32 * i < cols) {
-              if (kc == 0) {
+            if (EPI == EPI_OUT || 32 * i < cols) {
+              if (kc == kb0) {
                 tmem_ld32(acc + 32 * i, z[i]);
               } else {
 #pragma unroll
@@ -632,6 +638,10 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) z[i][j] = NAN;
         }
+      };
+      float z[COLS / 32][32];
+      if constexpr (LOGITS) {
+        collect(z, 0, ts.k_blocks);
         const bool live = t < M;
         const long long label = live ? a.tok.labels[t] : a.ignore;
         const long long at = label - a.n_first - n0;  // the label's column here
@@ -719,18 +729,13 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
                 make_float2(mx, rest);
         }
       } else if constexpr (EPI == EPI_PARTIAL) {
-        const bool there = ready();
-        const uint32_t acc = accumulator();
-        for (int c = 0; c < COLS && c < cols; c += 32) {
-          unsigned char *sl = next_slab();
-          float v[32];
-          if (there) {
-            tmem_ld32(acc + c, v);
-          } else {
+        const int kb0 = split * ts.split_blocks;
+        collect(z, kb0, min(kb0 + ts.split_blocks, ts.k_blocks));
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = NAN;
-          }
-          put_floats(sl, lane, v);
+        for (int c = 0; c < COLS; c += 32) {
+          if (c >= cols) break;
+          unsigned char *sl = next_slab();
+          put_floats(sl, lane, z[c / 32]);
           filled();
           const int r = m0 + quarter * 32;
           if (lane == 0 && r < a.M && (!a.low || r % VL_LOW < a.low)) {
@@ -738,55 +743,35 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
             store_commit();
           }
         }
-        if (there) release();
       } else {
-        // the tokens whose label is one of this warp's words, the first 32 of them in its
-        // lanes: asked for before the wait
+        // the tokens whose label is one of this warp's words
         const int word0 = a.m_first + m0 + quarter * 32;
-        int own = 0, own_end = 0, own_token = 0, own_label = 0;
-        float own_left = 0.0f;
-        if (sums && a.tok.by.first) {
+        int own = 0, own_end = 0;
+        if (sums && a.tok.by.first)
           own = a.tok.by.first[word0 / VL_GROUP], own_end = a.tok.by.first[word0 / VL_GROUP + 1];
-          if (own + lane < own_end) {
-            own_token = a.tok.by.token[own + lane], own_label = a.tok.by.label[own + lane];
-            own_left = a.label_left[own_token];
-          }
-        }
-        float z[COLS / 32][32];
-        if (sums && ready()) {
-          const uint32_t acc = accumulator();
 #pragma unroll
-          for (int i = 0; i < COLS / 32; ++i)
-            tmem_ld32(acc + 32 * i, z[i]);
-          release();
-        } else {
+        for (int i = 0; i < COLS / 32; ++i)
 #pragma unroll
-          for (int i = 0; i < COLS / 32; ++i)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) z[i][j] = ok ? 0.0f : NAN;
-        }
+          for (int j = 0; j < 32; ++j) z[i][j] = 0.0f;
+        collect(z, 0, ts.k_blocks);
         // what rounding left of dz at the label, times the token's row of h: two columns a
         // lane, summed over the tokens of a word, then through the slab to the word's own
         // lane.  7 us of a step of 128 tokens (887) on a 128256 x 4096 head, below the noise
         // of one of 4096 (12.7 ms), 15 % where thousands of tokens all have one label
         static_assert(EPI != EPI_OUT || COLS == 64, "two columns a lane");
-        const T *h = static_cast<const T *>(a.tok.rows) + n0 + 2 * lane;
-        while (own < own_end) {
-          const int n = min(32, own_end - own);
+        if (own < own_end) {
+          const T *h = static_cast<const T *>(a.tok.rows) + n0 + 2 * lane;
           float2 v = make_float2(0.0f, 0.0f);
-          auto row_of = [&](int i) -> uint32_t {
-            const long long token = __shfl_sync(~0u, own_token, i & 31);
-            if (i >= n || 2 * lane >= cols) return 0;
-            return *reinterpret_cast<const uint32_t *>(h + token * a.N);
-          };
-          uint32_t x[2] = {row_of(0), row_of(1)};  // two rows in flight
-          for (int i = 0; i < n; ++i) {
-            const int label = __shfl_sync(~0u, own_label, i);
-            const float left = __shfl_sync(~0u, own_left, i);
-            const float2 r = unpack2<T>(x[0]);
-            x[0] = x[1], x[1] = row_of(i + 2);
-            v.x = fmaf(left, r.x, v.x), v.y = fmaf(left, r.y, v.y);
-            if (i + 1 < n && __shfl_sync(~0u, own_label, i + 1) == label) continue;
+#pragma unroll 1
+          for (; own < own_end; ++own) {
+            const int label = a.tok.by.label[own], token = a.tok.by.token[own];
+            const float left = a.label_left[token];
+            if (2 * lane < cols) {
+              const float2 r =
+                  unpack2<T>(*reinterpret_cast<const uint32_t *>(h + (long long)token * a.N));
+              v.x = fmaf(left, r.x, v.x), v.y = fmaf(left, r.y, v.y);
+            }
+            if (own + 1 < own_end && a.tok.by.label[own + 1] == label) continue;
             float2 *through = reinterpret_cast<float2 *>(next_slab());
             through[lane] = v;
             __syncwarp();
@@ -799,11 +784,6 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
               }
             }
             v = make_float2(0.0f, 0.0f);
-          }
-          own += n;
-          if (own + lane < own_end) {
-            own_token = a.tok.by.token[own + lane], own_label = a.tok.by.label[own + lane];
-            own_left = a.label_left[own_token];
           }
         }
 #pragma unroll

@@ -104,3 +104,65 @@ def test_labels_outside_the_vocabulary_among_many():
             assert torch.isnan(dw).all() and torch.isnan(dh[7]).all()
             keep = torch.arange(t, device="cuda") != 7
             assert torch.equal(dh[keep], clean[keep])
+
+
+def _is_unbiased(got, want, steps):
+    """The mean relative error of n values of one sign: at most `steps` steps (2^-23) of the
+    sums, and what n roundings to nearest, each half a step of the type at most, leave of
+    their mean: more than 6 / sqrt(n) of that once in 3e7 draws (Hoeffding's bound)."""
+
+    n = want.numel()
+    mean = float(((got.double() - want) / want).mean())
+    tol = steps * 2.0 ** -23 + 6 * half_step(got.dtype) / n ** 0.5
+    assert abs(mean) <= tol, (mean, tol)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_weight_gradient_of_a_million_tokens(dtype):
+    """Sums of 2^20 products of one sign: a tensor core's accumulator truncates at every 16 of
+    them, so one over all would lose up to 65536 steps.  At most 16384 products run in one
+    accumulator here: 1024 steps, and 64 roundings where the sums are joined.  W is zero, so
+    that each p is 2^-6 and each dz exact."""
+    from easyfhe import plain
+
+    t, v, d = 1 << 20, 64, 2048
+    g = torch.Generator(device="cuda").manual_seed(1)
+    h = torch.empty((t, d), dtype=dtype, device="cuda")
+    want = torch.zeros(d, dtype=torch.float64, device="cuda")
+    for part in h.split(1 << 16):
+        part.copy_(torch.rand(part.shape, generator=g, device="cuda") + 0.5)
+        want += part.double().sum(0)
+    want /= t
+    w = torch.zeros((v, d), dtype=dtype, device="cuda")
+    labels = torch.full((t,), 3, device="cuda")
+    _, lse = plain.vocab_loss(h, w, labels)
+    _, dw = plain.vocab_loss_grad(h, w, labels, lse, torch.full((t,), 1.0 / t, device="cuda"),
+                                  need_hidden=False)
+    _is_unbiased(dw[0], want / 64, 1024 + 64)
+    _is_unbiased(dw[3], want * (-63 / 64), 1024 + 64)
+    assert torch.equal(dw[0], dw[63])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,d", [(120, 4096), (200, 4096), (250, 8192)])
+def test_hidden_gradient_over_half_a_million_words(dtype, t, d):
+    """As above, over the words: hidden states of zero, so that each p is 2^-19, and a label
+    whose word is zero.  Up to 1024 steps in one accumulator, and 32 joined."""
+    from easyfhe import plain
+
+    v = 1 << 19
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.empty((v, d), dtype=dtype, device="cuda")
+    want = torch.zeros(d, dtype=torch.float64, device="cuda")
+    for part in w.split(1 << 15):
+        part.copy_(torch.rand(part.shape, generator=g, device="cuda") + 0.5)
+    w[5] = 0.0
+    for part in w.split(1 << 15):
+        want += part.double().sum(0)
+    h = torch.zeros((t, d), dtype=dtype, device="cuda")
+    labels = torch.full((t,), 5, device="cuda")
+    _, lse = plain.vocab_loss(h, w, labels)
+    dh, _ = plain.vocab_loss_grad(h, w, labels, lse, torch.ones(t, device="cuda"),
+                                  need_weight=False)
+    _is_unbiased(dh[0], want / v, 1024 + 32)
+    _is_unbiased(dh[t - 1], want / v, 1024 + 32)
