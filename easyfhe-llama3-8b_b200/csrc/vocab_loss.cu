@@ -684,11 +684,13 @@ __global__ void __launch_bounds__(Block<CG>::threads, 1)
             for (int q = 0; q < 2; ++q) {
               float(&v)[32] = z[c / 32 + q];
               const int h = hit - c - 32 * q;
-              const float own = h >= 0 && h < 32 ? g * expm1f(pick(v, h) - lse) : 0.0f;
+              // with g = 0 all are 0, also where the logits are not finite
+              const float own =
+                  h >= 0 && h < 32 && g != 0.0f ? g * expm1f(pick(v, h) - lse) : 0.0f;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const float p = ex2((v[j] - lse) * kLog2e);
-                v[j] = g == 0.0f ? 0.0f : g * p;  // 0 too where the logits are not finite
+                v[j] = g == 0.0f ? 0.0f : g * p;
                 if (j == h) v[j] = own;
               }
               put_half<T>(sl, lane, q, v);

@@ -461,7 +461,8 @@ def vocab_loss_grad(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     gradient is rounded to the operands' type (f16: to no less than 2^-38 of the
     largest |grad_loss|), up to 64 tokens in two parts; from 65 tokens on
     what that leaves at the label still joins both gradients.  Rows of ignored tokens
-    contribute nothing and get zero, whatever they hold."""
+    contribute nothing and get zero, whatever they hold; so do tokens under a
+    grad_loss of zero whose hidden state is finite."""
 
     index, t, v, d = _loss_args("vocab_loss_grad", hidden, weight, labels, lse=lse,
                                 grad_loss=grad_loss)

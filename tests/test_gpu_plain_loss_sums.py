@@ -166,3 +166,21 @@ def test_hidden_gradient_over_half_a_million_words(dtype, t, d):
                                   need_weight=False)
     _is_unbiased(dh[0], want / v, 1024 + 32)
     _is_unbiased(dh[t - 1], want / v, 1024 + 32)
+
+
+@pytest.mark.parametrize("t", [9, 64, 100, 300, 1100])
+def test_no_upstream_gradient_no_gradient(t):
+    """A token whose finite operands overflow its logits, under an upstream gradient of zero:
+    its rows are zero and the others' what they are beside a harmless token."""
+    from easyfhe import plain
+
+    h, w, labels, grad = _inputs(t, 400, 64, BF, ignored=0.0)
+    grad[2] = 0.0
+    _, lse = plain.vocab_loss(h, w, labels)
+    want = plain.vocab_loss_grad(h, w, labels, lse, grad)
+    assert not want[0][2].any()
+    h[2] = 3e38
+    _, lse = plain.vocab_loss(h, w, labels)
+    assert not torch.isfinite(lse[2])
+    got = plain.vocab_loss_grad(h, w, labels, lse, grad)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
