@@ -10,8 +10,9 @@ Every call is asynchronous on the current stream of its tensors' device and
 can be captured into a CUDA graph; scratch and outputs come from torch's
 allocator on that stream.  Tensors used on a stream other than the one they
 were made on are the caller's to order, as with any torch operation.  Gradients
-are explicit calls: nothing here records an autograd graph, and tensors that
-require a gradient are refused unless gradients are switched off.  Arguments
+are explicit calls: nothing here records an autograd graph or carries tangents,
+and tensors that require a gradient are refused unless gradients are switched
+off, dual tensors of forward-mode differentiation always.  Arguments
 are checked before anything launches: ValueError for shapes, types, strides
 and devices (there is no CPU fallback).
 """
@@ -19,10 +20,10 @@ and devices (there is no CPU fallback).
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
-
-import struct
+from torch.autograd import forward_ad
 
 from ._native import call, check, lib
 
@@ -33,11 +34,18 @@ _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+def _dual(t) -> bool:
+    """A tensor with a tangent; there are none outside forward_ad.dual_level()."""
+
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _plain_tensor(t, index: int) -> bool:
     """A strided CUDA tensor on device `index` that asks for no gradient."""
 
     return isinstance(t, torch.Tensor) and t.get_device() == index and not t.is_neg() \
-        and not (t.requires_grad and torch.is_grad_enabled()) and t.layout is torch.strided
+        and not (t.requires_grad and torch.is_grad_enabled()) and t.layout is torch.strided \
+        and not _dual(t)
 
 
 def _refuse(what: str, index: int | None, **tensors) -> None:
@@ -55,6 +63,9 @@ def _refuse(what: str, index: int | None, **tensors) -> None:
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what}: {name} requires a gradient, which this call does not "
                              "record (use the explicit gradient call under torch.no_grad())")
+        if _dual(t):
+            raise ValueError(f"{what}: {name} is a dual tensor, whose tangent this call does "
+                             "not carry (take forward_ad.unpack_dual(...).primal)")
         if not _plain_tensor(t, t.get_device()):
             raise ValueError(f"{what}: {name} is not a plain strided tensor")
 

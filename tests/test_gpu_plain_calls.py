@@ -138,3 +138,30 @@ def test_copies_of_plans_and_weights_stand_alone():
     w.packed.zero_()
     assert torch.equal(plain.rope(q, positions=pos, plan=plan2), want[0])
     assert torch.equal(plain.q4_matvec(x, w2), want[1])
+
+
+def test_dual_tensors_are_refused():
+    from torch.autograd import forward_ad
+
+    from easyfhe import plain
+
+    plan = plain.RopePlan(64)
+    w4 = plain.quantize_q4(torch.randn((50, 64), device="cuda"), group=64)
+    h, lab = torch.randn((5, 64), device="cuda").bfloat16(), torch.arange(5, device="cuda")
+    loss, lse = plain.vocab_loss(h, h, lab)
+    one = torch.ones_like(loss)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: plain.rope(dual(h)[None], positions=lab[:1], plan=plan),
+                     lambda: plain.rope(h[None], dual(h)[None], positions=lab[:1], plan=plan),
+                     lambda: plain.rope_grad(dual(h)[None], positions=lab[:1], plan=plan),
+                     lambda: plain.q4_matvec(dual(h), w4), lambda: plain.q4_codes(dual(h)),
+                     lambda: plain.vocab_loss(dual(h), h, lab),
+                     lambda: plain.vocab_loss(h, dual(h), lab),
+                     lambda: plain.vocab_loss_grad(h, h, lab, dual(lse), one),
+                     lambda: plain.vocab_loss_grad(h, h, lab, lse, dual(one))):
+            with pytest.raises(ValueError, match="dual"):
+                call()
+        assert torch.equal(plain.vocab_loss(h, h, lab)[0], loss)

@@ -145,3 +145,22 @@ def test_host_tensors_are_refused():
         plain.pack_q4(torch.zeros(2, 64, dtype=torch.uint8), h[:, :1])
     with pytest.raises(ValueError, match="weight"):
         plain.q4_matvec(h, h)
+
+
+def test_dual_tensors_are_refused():
+    """A tangent would be lost without a word: the output would have none."""
+    import torch
+    from torch.autograd import forward_ad
+
+    from easyfhe import plain
+
+    x = torch.zeros(2, 8)
+    assert plain._plain_tensor(x, -1)  # as on a device of that number
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert not plain._plain_tensor(dual, -1)
+        assert plain._plain_tensor(forward_ad.unpack_dual(dual).primal, -1)
+        assert plain._plain_tensor(x, -1)
+        with torch.no_grad():
+            assert not plain._plain_tensor(dual, -1)
+    assert plain._plain_tensor(x, -1)
