@@ -408,6 +408,32 @@ class ReferenceSession:
 # ---------------------------------------------------------------------------
 
 
+PROMPT, HIDDEN = 128, 4096  # tokens and features of a prefill
+
+
+def _check_answer(check: bool, head, tokens) -> None:
+    """Refuse before anything runs what answer_check could not use after it."""
+
+    import torch
+
+    if head is None:
+        if tokens is not None:
+            raise ValueError("tokens without a head to score them")
+        return
+    if not check:
+        raise ValueError("a head with check=False: the answer is one of the checks")
+    if tokens is None:
+        raise ValueError("a head without the prompt's tokens")
+    words, hidden = head.weight.shape
+    t = torch.as_tensor(tokens)
+    if tuple(t.shape) != (PROMPT,) or hidden != HIDDEN:
+        raise ValueError(f"tokens of shape {tuple(t.shape)} and a head of {hidden} features for "
+                         f"hidden states of {PROMPT} x {HIDDEN}")
+    if t.is_floating_point() or t.dtype == torch.bool or int(t.min()) < 0 \
+            or int(t.max()) >= words:
+        raise ValueError(f"tokens outside the head's {words} words")
+
+
 def run_layer0(*, warmup: int = 1, repetitions: int = 1, seed: int = 26081461,
                extra_args=(), check: bool = True, check_device=None,
                head: ClientHead | None = None, tokens=None) -> dict:
@@ -418,6 +444,7 @@ def run_layer0(*, warmup: int = 1, repetitions: int = 1, seed: int = 26081461,
     ``"answer"``, the client's answer from the decrypted layer against the plain
     one."""
 
+    _check_answer(check, head, tokens)
     import_reference()
     from llama3fhe.application import runner
 
@@ -574,6 +601,7 @@ def run_prefill(num_layers: int = 32, *, seed: int = 26081461, check: bool = Tru
     RMSNorm, and no boundary is decrypted until the end.  ``check_device``,
     ``head`` and ``tokens`` as in run_layer0."""
 
+    _check_answer(check, head, tokens)
     import_reference()
     from llama3fhe import Llama3CKKSConfig
     from llama3fhe.application import args as ref_args
@@ -667,7 +695,7 @@ if __name__ == "__main__":
     if "--answer" in sys.argv[1:]:  # the client's answer too, on a seeded head and prompt
         rng = np.random.default_rng(26081461)
         extra = {"check_device": "cuda", "head": synthetic_head(),
-                 "tokens": rng.integers(0, 128256, 128)}
+                 "tokens": rng.integers(0, 128256, PROMPT)}
     r = run_layer0(**extra)
     print(json.dumps({"s_per_layer": r["s_per_layer"], "checks": r.get("checks"),
                       **({"answer": r["answer"]} if "answer" in r else {}),

@@ -164,3 +164,32 @@ def test_dual_tensors_are_refused():
         with torch.no_grad():
             assert not plain._plain_tensor(dual, -1)
     assert plain._plain_tensor(x, -1)
+
+
+@pytest.mark.parametrize("run", ["run_layer0", "run_prefill"])
+def test_an_answer_that_cannot_be_given_is_refused_first(run, monkeypatch):
+    """Before the encrypted layers run: a head without tokens, with tokens that are not the
+    prompt's, or with the checks off."""
+    from types import SimpleNamespace
+
+    import torch
+
+    import llama3_layer
+
+    def reached():
+        raise AssertionError("the layers would have run")
+
+    monkeypatch.setattr(llama3_layer, "import_reference", reached)
+    run = getattr(llama3_layer, run)
+    head = SimpleNamespace(weight=torch.empty((1000, 4096), device="meta"))
+    small = SimpleNamespace(weight=torch.empty((1000, 64), device="meta"))
+    tokens = torch.arange(128)
+    for kw in ({"head": head}, {"tokens": tokens}, {"head": head, "tokens": tokens, "check": False},
+               {"head": head, "tokens": tokens[:127]}, {"head": head, "tokens": tokens + 873},
+               {"head": head, "tokens": tokens - 1}, {"head": head, "tokens": tokens.float()},
+               {"head": small, "tokens": tokens}):
+        with pytest.raises(ValueError):
+            run(**kw)
+    for kw in ({}, {"head": head, "tokens": tokens}, {"head": head, "tokens": list(range(128))}):
+        with pytest.raises(AssertionError, match="would have run"):
+            run(**kw)
