@@ -19,10 +19,10 @@
 // output's address), and registers for five blocks of 256 threads on an SM (four
 // with two heads in flight per thread: 129 us).
 // The angle of a far position needs more than binary32: p f is formed in binary64
-// and reduced there to a fraction of a turn in [-1/2, 1/2], whose sine and cosine
-// are then taken in binary32 (the reduction's error is 2^-52 of the turns, the
-// rounding of the fraction 2^-25 of a turn); binary64 inputs take binary64 sines of
-// p f.
+// and reduced there to a fraction of a turn in [-1/2, 1/2] (off by 2^-52 of the turns).
+// Heads of 16 bits take its sine and cosine in binary32 (the rounding of the fraction is
+// 2^-26 of a turn at most, far below their own step); binary32 heads, which would feel that,
+// take them in binary64 and round once; binary64 heads take binary64 sines of p f.
 #include "plain.h"
 
 #include <cuda_bf16.h>
@@ -87,19 +87,29 @@ __device__ __forceinline__ __nv_bfloat16 from_wide<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// (cos, sin) of p f
-__device__ __forceinline__ void turn_of(double p, double f, float factor, int sign, float2 &o) {
+// m (cos, sin) of p f for heads of type T
+template <class T>
+__device__ __forceinline__ void turn_of(double p, double f, double factor, int sign,
+                                        typename Wide<T>::V2 &o) {
   constexpr double kInv2Pi = 0.15915494309189533577;
-  double t = p * f * kInv2Pi;
-  t -= rint(t);
-  float s, c;
-  sincospif(2.0f * (float)t, &s, &c);
-  o = make_float2(c * factor, (float)sign * s * factor);
-}
-__device__ __forceinline__ void turn_of(double p, double f, double factor, int sign, double2 &o) {
-  double s, c;
-  sincos(p * f, &s, &c);
-  o = make_double2(c * factor, (double)sign * s * factor);
+  if constexpr (std::is_same<T, double>::value) {
+    double s, c;
+    sincos(p * f, &s, &c);
+    o = make_double2(c * factor, (double)sign * s * factor);
+    return;
+  } else {
+    double t = p * f * kInv2Pi;
+    t -= rint(t);
+    if constexpr (std::is_same<T, float>::value) {
+      double s, c;
+      sincospi(2.0 * t, &s, &c);
+      o = make_float2((float)(c * factor), (float)((double)sign * s * factor));
+    } else {
+      float s, c;
+      sincospif(2.0f * (float)t, &s, &c);
+      o = make_float2(c * (float)factor, (float)sign * s * (float)factor);
+    }
+  }
 }
 
 // two roundings at once
@@ -142,7 +152,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 5)
       const double p = a.pos64 ? (double)static_cast<const long long *>(a.pos)[at]
                                : (double)static_cast<const int *>(a.pos)[at];
       W2 cs;
-      turn_of(p, a.freqs[j], (W)a.factor, a.sign, cs);
+      turn_of<T>(p, a.freqs[j], a.factor, a.sign, cs);
       cosines[i] = cs.x;
       sines[i] = cs.y;
     }
