@@ -78,3 +78,31 @@ def test_infinities_in_long_rows(rows):
             assert torch.equal(torch.isnan(y[-1]), torch.isnan(want)), at
             ok = ~torch.isnan(want)
             assert torch.equal(y[-1, ok].double(), want[ok]), at
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,k,group,zeros", [
+    (33, 14336, 64, True), (33, 70001, 128, False), (18, 131072, 32, True), (33, 131072, 64, False),
+    (1001, 4096, 128, False), (14300, 14336, 128, False), (28500, 4097, 64, True),
+    (28500, 24000, 32, False), (14300, 131072, 128, False)])
+@pytest.mark.parametrize("rows", [1, 2, 4, 11, 33])
+def test_integers_are_exact(dtype, n, k, group, zeros, rows):
+    """Integers from -4 to 4 times weights from -15 to 15 under scales of 1: every sum of them
+    is an integer below 2^24, which binary32 holds in whatever order it is formed.  A lost or
+    doubled column, tile, warp or block shows."""
+    from easyfhe import plain
+
+    g = torch.Generator(device="cuda").manual_seed(k + rows)
+    codes = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.ones((n, -(-k // group)), device="cuda", dtype=torch.float16)
+    z = torch.randint(0, 16, scales.shape, generator=g, device="cuda", dtype=torch.uint8) \
+        if zeros else None
+    x = torch.randint(-4, 5, (rows, k), generator=g, device="cuda")
+    assert 4 * 15 * k < 2 ** 24
+    w = plain.pack_q4(codes, scales, z, group=group)
+    y = plain.q4_matvec(x.to(dtype), w, out_dtype=torch.float32)
+    for n0 in range(0, n, 2000):
+        part = slice(n0, n0 + 2000)
+        want = x.double() @ q4_weight64(codes[part], scales[part],
+                                        None if z is None else z[part], group).T
+        assert torch.equal(y[:, part].double(), want), n0
