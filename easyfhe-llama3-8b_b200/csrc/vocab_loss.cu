@@ -38,12 +38,13 @@
 // loses.  fp16 cannot hold g p of a rare word, so there dz is scaled by a power of two
 // that brings the largest |g| to 2^14 and the products are scaled back in binary32.
 //
-// Measured on a 128256 x 4096 head in bf16: the score of 128 tokens 174-181 us (W read
-// once at 88-92 % of copy bandwidth); a training step on them 870 us = that + 182 (dz:
-// W again) + 155 (dh: W a third time) + 284 (dW; clearing as many bytes takes 275); a
-// step on 4096 tokens 12.4-13.1 ms, 1.19-1.25 PFLOP/s over the four products of the counted
-// tokens, under the power cap (cuBLAS sustains 1.385).  dh, dW and the next piece's logits
-// side by side on clusters of their own were no faster (672 against 660 us).
+// Measured on a 128256 x 4096 head in bf16: the score of 128 tokens 176-182 us (W read
+// once at 88-91 % of copy bandwidth); a training step on them 855-905 us, its launches one by
+// one 190 (logits) + 184 (dz: W again) + 156 (dh: W a third time) + 305 (dW; clearing as many
+// bytes takes 350) + 23 (the small ones); a step on 4096 tokens 12.5-13.5 ms, 1.15-1.24 PFLOP/s
+// over the four products of the counted tokens, under the power cap (cuBLAS sustains 1.385).
+// dh, dW and the next piece's logits side by side on clusters of their own were no faster
+// (672 against 660 us).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>

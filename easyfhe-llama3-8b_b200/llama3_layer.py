@@ -324,7 +324,8 @@ def synthetic_head(seed: int = 26081461, words: int = 128256, hidden: int = 4096
 def answer_check(decoded, reference, head: ClientHead, tokens) -> dict:
     """How far the decryption error of hidden states moves the client's answer:
     the prompt's score and next token from the decrypted and from the plain
-    states, and the score's change to first order in the error."""
+    states, and the score's change to first order in the error.  Next tokens and
+    logits are the 4-bit head's on both sides, scores the bf16 head's."""
 
     import torch
 

@@ -516,7 +516,8 @@ int b2f_q4_quantize(const void *w, int dtype, int64_t ld, int64_t N, int64_t K, 
  * read once per 16 rows (4 of f32; fewer of long rows: what shared memory holds
  * of x).  Binary32 rows and one or two rows of a 16-bit type may
  * be taken as fixed-point numbers, off by at most 2^-30 of the largest of their 64
- * columns; otherwise every value of x enters exactly. */
+ * columns (and NaN under a zero weight where scale times value reaches 2^134, which any
+ * other weight overflows); otherwise every value of x enters exactly. */
 int b2f_q4_matvec(const void *x, int dtype, int64_t ldx, int64_t rows, const void *packed,
                   int scale_dtype, int zeros, int64_t N, int64_t K, int group, void *y,
                   int out_f32, void *stream);
