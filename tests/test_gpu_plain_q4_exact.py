@@ -106,3 +106,29 @@ def test_integers_are_exact(dtype, n, k, group, zeros, rows):
         want = x.double() @ q4_weight64(codes[part], scales[part],
                                         None if z is None else z[part], group).T
         assert torch.equal(y[:, part].double(), want), n0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinities_in_rows_and_results_of_16_bits(dtype):
+    """As above with y in x's type, from rows that are views."""
+    from easyfhe import plain
+
+    n, k = 40001, 320
+    g = torch.Generator(device="cuda").manual_seed(3)
+    codes = torch.randint(6, 11, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.full((n, k // 64), 2.0 ** -6, device="cuda", dtype=torch.float16)
+    w = plain.pack_q4(codes, scales, group=64)
+    w64 = q4_weight64(codes, scales, None, 64)
+    wide = torch.randn((2, 407), generator=g, device="cuda").to(dtype)
+    for at in ({300: 1}, {0: -1, 319: -1}, {7: 1, 9: 1, 200: -1}):
+        x = wide.clone()[:, 3:323]
+        clean = plain.q4_matvec(x, w)
+        for column, sign in at.items():
+            x[1, column] = sign * INF
+        y = plain.q4_matvec(x, w)
+        assert y.dtype == dtype and torch.equal(y[0], clean[0])
+        cols = torch.tensor(sorted(at), device="cuda")
+        want = (w64[:, cols] * x[1, cols].double()).sum(1)
+        assert torch.equal(torch.isnan(y[1]), torch.isnan(want)), at
+        ok = ~torch.isnan(want)
+        assert torch.equal(y[1, ok].double(), want[ok]), at
